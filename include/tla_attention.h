@@ -394,17 +394,104 @@ int tla_generate_greedy(tla_engine* e, const tla_model* m, float* key_cache_dev,
                         float* value_cache_dev, const int* prompt_host, int n_prompt, int n_gen,
                         int flags, int* tokens_host);
 
+/* ---- serving over a paged cache (no reference counterpart: the reference
+ *      holds one sequence) ------------------------------------------------ */
+
+/* Element types of a paged cache: ggml_type ids. */
+enum tla_kv_type { TLA_KV_F32 = 0, TLA_KV_F16 = 1, TLA_KV_BF16 = 30 };
+
+/* Keys and values of many sequences in pages of page_size positions (a power
+ * of two up to 1024).  Element (layer, page, row, kv_head, j) is at
+ *     layer * layer_stride + page * page_stride + (row * n_head_kv + kv_head) * 64 + j
+ * of key_pages and of value_pages.  Position p of sequence s is row
+ * p % page_size of page table_dev[s * table_stride + p / page_size], in every
+ * layer.  An entry outside [0, n_pages) is an absent page (a sequence whose
+ * oldest pages were given back, say): nothing is written to it, and its
+ * positions are not attended to.  Sequences may share pages that they only read;
+ * a row that one call appends to twice holds either.  Rows past a sequence's
+ * end, and entries of the table past its last page, are never read as values. */
+typedef struct tla_paged_cache {
+    void* key_pages;      /* device, 16-byte aligned */
+    void* value_pages;
+    int type;             /* tla_kv_type */
+    int page_size;
+    int n_pages;          /* of one layer */
+    size_t page_stride;   /* elements, a multiple of 8; 0: page_size * n_head_kv * 64 */
+    size_t layer_stride;  /* elements, a multiple of 8; 0: n_pages * page_stride */
+    const int* table_dev; /* [n_seq][table_stride] page numbers */
+    int table_stride;
+} tla_paged_cache;
+
+/* Zero-filled, dense key and value pages for the engine's layers: sets every
+ * field of *cache but the table's (left NULL and 0).  Free key_pages and
+ * value_pages with tla_free. */
+int tla_paged_cache_alloc(tla_engine* e, int n_pages, int page_size, int type, tla_paged_cache* cache);
+
+/* Appends the new tokens of n_seq sequences to one layer's pages: sequence s
+ * brings n_tok_host[s] >= 0 tokens (n_tok_host NULL: one each) at positions
+ * pos_host[s] .. .  k_dev, v_dev [total tokens][n_head_kv][64] fp32, sequences
+ * one after the other, 16-byte aligned.  With TLA_ROTATE, k is rotated at its
+ * token's position, with the bits of tla_rope; F16 and BF16 elements are then
+ * rounded to nearest.  pos + n_tok at most n_ctx and table_stride * page_size; up
+ * to 256 sequences. */
+int tla_paged_append(tla_engine* e, const tla_paged_cache* cache, int n_seq, const int* pos_host,
+                     const int* n_tok_host, int layer, int flags, const float* k_dev, const float* v_dev);
+
+/* Causal attention of the new tokens (appended before, as above) over their
+ * sequences' pages: token t of sequence s attends to positions 0 .. pos_host[s] +
+ * t, those of absent pages left out; a row that is left none is 0.  Any mix of
+ * single tokens and chunks of prompts.  q_dev, out_dev [total tokens][n_head]
+ * [64] fp32, 16-byte aligned (they may be the same); TLA_ROTATE rotates q.
+ * fp32 accuracy for every element type; keys and values that are seen and
+ * not finite give what fp32 gives.  Limits as tla_paged_append's. */
+int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, const int* pos_host,
+                        const int* n_tok_host, int layer, int flags, float* out_dev, const float* q_dev);
+
+/* Rules on the logits of a batch, row by row: NULL where there is none of a
+ * kind.  Device pointers. */
+typedef struct tla_logit_rules {
+    /* Tokens already said, in any order, [n_seq][history_stride], the first
+     * history_len[s] of row s (clamped to the stride); ones outside [0, n_vocab)
+     * do not count.  penalties [n_seq][3]: repetition r, presence a and
+     * frequency f.  A token said c > 0 times: x = x > 0 ? x / r : x * r, then
+     * x = x - (c * f + a). */
+    const int* history_dev;
+    const int* history_len_dev;
+    int history_stride;
+    const float* penalties_dev;
+    /* Then x = x + bias, for the tokens of a list [n_seq][bias_stride], its
+     * first bias_len[s]; the last of several entries for a token counts. */
+    const int* bias_token_dev;
+    const float* bias_value_dev;
+    const int* bias_len_dev;
+    int bias_stride;
+    /* Then x = -inf for a token j whose bit j % 32 of word j / 32 is 0,
+     * [n_seq][mask_stride] words. */
+    const unsigned* mask_dev;
+    int mask_stride;
+} tla_logit_rules;
+
+/* Applies the rules (NULL: none) to logits_dev [n_seq][n_vocab] into out_dev
+ * (which may be the same) and, unless tokens_dev is NULL, writes each row's
+ * first index of the largest result to tokens_dev [n_seq]: -1 where nothing
+ * above -inf is left; a NaN never wins.  Each operation is rounded to fp32 on
+ * its own.  Up to 65536 rows, n_vocab up to 2^28. */
+int tla_logits_process(tla_engine* e, int n_seq, int n_vocab, const tla_logit_rules* rules, float* out_dev,
+                       const float* logits_dev, int* tokens_dev);
+
 /* ---- measurement hooks (no reference counterpart) ------------------- */
 enum tla_kernel_id {
     TLA_KERNEL_DECODE = 0,  /* split-KV decode attention (and forward()'s
                                short-context attention + W_o): RoPE + append +
                                attention + split merge, one launch           */
     TLA_KERNEL_PREFILL = 1, /* causal MFMA prefill attention (short prompts: with
-                               their RoPE + append, one launch)              */
-    TLA_KERNEL_APPEND = 2,  /* prefill RoPE + cache append, as its own launch */
+                               their RoPE + append, one launch); tla_paged_attention */
+    TLA_KERNEL_APPEND = 2,  /* prefill RoPE + cache append, as its own launch;
+                               tla_paged_append                               */
     TLA_KERNEL_GEMV = 3,    /* projections: matmul / attn_qkv / attn_out /
                                ffn / classifier                              */
-    TLA_KERNEL_COUNT = 4
+    TLA_KERNEL_LOGITS = 4,  /* rules on logits                                */
+    TLA_KERNEL_COUNT = 5
 };
 /* When enabled, HIP events bracket every launch of each kernel on the
  * engine's stream; tla_profile_read sums their durations (ms) since the

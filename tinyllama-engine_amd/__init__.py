@@ -13,6 +13,9 @@ Interfaces mirrored (reference files):
     Engine.decode      batched / multi-layer decode (one attention() per
                        (sequence, layer))
     Engine.prefill     the prompt loop src/generate.cpp:56-59, batched
+    Engine.paged_cache / paged_append / paged_attention / logits_process
+                       a serving step of many sequences over pages of keys and
+                       values (no counterpart)
     Engine.kv_cache    RunState::key_cache / value_cache src/run_state.h:93-101
     Engine.matmul / rmsnorm / vec_add / silu / elementwise_mul / ffn_swiglu
                        the ops of src/ops.h:64-66, 95-96, 118, 131, 143, 232-235
@@ -45,7 +48,9 @@ TLA_ROTATE = 1
 TLA_BATCH_PROMPT = 2
 TLA_KV_IN_CACHE = 4
 
-KERNEL_DECODE, KERNEL_PREFILL, KERNEL_APPEND, KERNEL_GEMV = range(4)
+KERNEL_DECODE, KERNEL_PREFILL, KERNEL_APPEND, KERNEL_GEMV, KERNEL_LOGITS = range(5)
+# element types of a paged cache: ggml_type ids
+KV_F32, KV_F16, KV_BF16 = 0, 1, 30
 # weight formats: the reference's ggml_type ids (src/gguf.h:23-32)
 W_F32, W_F16, W_Q4_0, W_Q8_0, W_Q6_K = 0, 1, 2, 8, 14
 OPT_DECODE_SPLIT, OPT_DECODE_PLAN, OPT_DECODE_GROUP = 0, 1, 2
@@ -101,6 +106,24 @@ class Model(C.Structure):
                 ("token_embd", _vp), ("type_embd", C.c_int), ("output_norm", _vp),
                 ("output", _vp), ("type_output", C.c_int), ("layers", C.POINTER(LayerWeights))]
 
+
+class PagedCache(C.Structure):
+    """tla_paged_cache: pages of keys and values and the sequences' page table
+    (device addresses; strides in elements, 0: dense)."""
+
+    _fields_ = [("key_pages", _vp), ("value_pages", _vp), ("type", C.c_int), ("page_size", C.c_int),
+                ("n_pages", C.c_int), ("page_stride", C.c_size_t), ("layer_stride", C.c_size_t),
+                ("table", _vp), ("table_stride", C.c_int)]
+
+
+class LogitRules(C.Structure):
+    """tla_logit_rules: device addresses, None for a kind that there is none of."""
+
+    _fields_ = [("history", _vp), ("history_len", _vp), ("history_stride", C.c_int), ("penalties", _vp),
+                ("bias_token", _vp), ("bias_value", _vp), ("bias_len", _vp), ("bias_stride", C.c_int),
+                ("mask", _vp), ("mask_stride", C.c_int)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/tla_attention.h
 SIGNATURES = {
     "tla_last_error": (C.c_char_p, []),
@@ -148,6 +171,11 @@ SIGNATURES = {
                                      _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t]),
     "tla_prefill": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                               _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tla_paged_cache_alloc": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.POINTER(PagedCache)]),
+    "tla_paged_append": (C.c_int, [_vp, C.POINTER(PagedCache), C.c_int, _vp, _vp, C.c_int, C.c_int, _vp, _vp]),
+    "tla_paged_attention": (C.c_int, [_vp, C.POINTER(PagedCache), C.c_int, _vp, _vp, C.c_int, C.c_int, _vp,
+                                      _vp]),
+    "tla_logits_process": (C.c_int, [_vp, C.c_int, C.c_int, C.POINTER(LogitRules), _vp, _vp, _vp]),
     "tla_profile_enable": (C.c_int, [_vp, C.c_int]),
     "tla_profile_read": (C.c_int, [_vp, C.c_int, C.POINTER(C.c_double),
                                    C.POINTER(C.c_longlong)]),
@@ -308,6 +336,46 @@ class Engine:
         _check(lib().tla_prefill(self.h, pos0, n_tok, layer0, n_step_layers,
                                  TLA_ROTATE if rotate else 0, out, q, k, v, key_cache,
                                  value_cache), "tla_prefill")
+
+    # ---- serving over a paged cache ---------------------------------------------
+    def paged_cache(self, n_pages: int, page_size: int, kv_type: int = KV_F16) -> PagedCache:
+        """Zeroed pages for the engine's layers; set table and table_stride, free with
+        free_paged_cache."""
+        c = PagedCache()
+        _check(lib().tla_paged_cache_alloc(self.h, n_pages, page_size, kv_type, C.byref(c)),
+               "tla_paged_cache_alloc")
+        return c
+
+    def free_paged_cache(self, cache: PagedCache):
+        for p in (cache.key_pages, cache.value_pages):
+            _check(lib().tla_free(self.h, p), "tla_free")
+        cache.key_pages = cache.value_pages = None
+
+    @staticmethod
+    def _batch(pos, n_tok):
+        """pos and n_tok (None: one token each) as int32 arrays of one length."""
+        pos = np.ascontiguousarray(pos, dtype=np.int32).reshape(-1)
+        if n_tok is None:
+            return pos, None, None
+        n_tok = np.ascontiguousarray(n_tok, dtype=np.int32).reshape(-1)
+        if n_tok.size != pos.size:
+            raise ValueError(f"{pos.size} positions, {n_tok.size} token counts")
+        return pos, n_tok, n_tok.ctypes.data
+
+    def paged_append(self, cache: PagedCache, pos, n_tok, layer: int, k: int, v: int, rotate: bool = True):
+        pos, n_tok, n_ptr = self._batch(pos, n_tok)
+        _check(lib().tla_paged_append(self.h, C.byref(cache), pos.size, pos.ctypes.data, n_ptr, layer,
+                                      TLA_ROTATE if rotate else 0, k, v), "tla_paged_append")
+
+    def paged_attention(self, cache: PagedCache, pos, n_tok, layer: int, out: int, q: int, rotate: bool = True):
+        pos, n_tok, n_ptr = self._batch(pos, n_tok)
+        _check(lib().tla_paged_attention(self.h, C.byref(cache), pos.size, pos.ctypes.data, n_ptr, layer,
+                                         TLA_ROTATE if rotate else 0, out, q), "tla_paged_attention")
+
+    def logits_process(self, n_seq: int, n_vocab: int, rules: LogitRules | None, out: int, logits: int,
+                       tokens: int | None = None):
+        _check(lib().tla_logits_process(self.h, n_seq, n_vocab, C.byref(rules) if rules else None, out, logits,
+                                        tokens), "tla_logits_process")
 
     # ---- projections either side of the attention block -------------------------
     def matmul(self, out: int, w: int, x: int, rows: int, cols: int, wtype: int):

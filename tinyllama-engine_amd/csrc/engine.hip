@@ -15,6 +15,8 @@
 
 
 #include "batch.h"
+#include "logits.h"
+#include "paged.h"
 #include "prefill.h"
 #include "tla_internal.h"
 
@@ -135,6 +137,10 @@ struct tla_engine {
     size_t kvp_bytes = 0;
     float* pf_part = nullptr;     // its states of workgroups that share a query tile
     int* pf_counters = nullptr;   // and their arrivals, zero between launches
+    unsigned long long* best = nullptr;  // logits: the best of each slice of each row
+    size_t best_bytes = 0;
+    int* best_counters = nullptr;        // and their arrivals, zero between launches
+    size_t n_best_counters = 0;
     int* argmax_slot = nullptr;
     unsigned long long* amax_keys = nullptr;  // kAmaxSlots keys (tla_matmul_argmax)
     long long opt_split = 0;
@@ -249,21 +255,20 @@ int ensure_ws(tla_engine* e, size_t bytes)
     return TLA_OK;
 }
 
-// Arrival counters for `units` (unit, kv head group) pairs.  Zeroed once
-// when (re)allocated (by a kernel: no memset node); the decode kernel returns
-// every counter it uses to zero.
-int ensure_counters(tla_engine* e, size_t units)
+// At least `want` arrival counters.  Zeroed once when (re)allocated (by a
+// kernel: no memset node); a launch returns every counter it uses to zero.
+int ensure_counters(tla_engine* e, int** counters, size_t& have, size_t want)
 {
-    if (units <= e->n_counters) return TLA_OK;
+    if (want <= have) return TLA_OK;
     TLA_HIP(hipStreamSynchronize(e->stream));
-    if (e->counters) TLA_HIP(hipFree(e->counters));
-    e->counters = nullptr;
-    e->n_counters = 0;
-    const size_t n = std::max<size_t>(units, 1024);
-    TLA_HIP(hipMalloc(&e->counters, n * sizeof(int)));
-    TLA_HIP(launch_zero(e->counters, n * sizeof(int), e->stream));
+    if (*counters) TLA_HIP(hipFree(*counters));
+    *counters = nullptr;
+    have = 0;
+    const size_t n = std::max<size_t>(want, 1024);
+    TLA_HIP(hipMalloc(counters, n * sizeof(int)));
+    TLA_HIP(launch_zero(*counters, n * sizeof(int), e->stream));
     TLA_HIP(hipStreamSynchronize(e->stream));
-    e->n_counters = n;
+    have = n;
     return TLA_OK;
 }
 
@@ -434,7 +439,7 @@ int tla_engine_create(const tla_config* cfg, int device, tla_engine** out)
     // Every kernel's code object is loaded now, not at its first launch (a
     // load allocates device memory: tla_decode_noalloc's first call would).
     for (hipError_t (*load)() : {load_decode_code, load_prefill_code, load_gemv_code, load_batch_code,
-                                 load_product_code, load_small_ops_code}) {
+                                 load_product_code, load_paged_code, load_logits_code, load_small_ops_code}) {
         const hipError_t lerr = load();
         if (lerr != hipSuccess)
             return bail(fail(TLA_ERR_DEVICE, "loading kernel code: %s", hipGetErrorString(lerr)));
@@ -464,6 +469,8 @@ int tla_engine_destroy(tla_engine* e)
     if (e->part) (void)hipFree(e->part);
     if (e->kvp) (void)hipFree(e->kvp);
     if (e->pf_part) (void)hipFree(e->pf_part);
+    if (e->best) (void)hipFree(e->best);
+    if (e->best_counters) (void)hipFree(e->best_counters);
     if (e->argmax_slot) (void)hipFree(e->argmax_slot);
     if (e->amax_keys) (void)hipFree(e->amax_keys);
     if (e->rope) (void)hipFree(e->rope);
@@ -1098,7 +1105,7 @@ int decode_impl(tla_engine* e, bool fixed_scratch, int n_seq, const int* pos_hos
             p.counters = reinterpret_cast<int*>(static_cast<char*>(e->scratch) + kScratchPartBytes);
         } else {
             if (int rc = ensure_ws(e, bytes)) return rc;
-            if (int rc = ensure_counters(e, n_counters)) return rc;
+            if (int rc = ensure_counters(e, &e->counters, e->n_counters, n_counters)) return rc;
             p.part = static_cast<float*>(e->ws);
             p.counters = e->counters;
         }
@@ -1266,6 +1273,190 @@ int tla_prefill(tla_engine* e, int pos0, int n_tok, int layer0, int n_step_layer
                         [&] { return launch_prefill_attention(p, e->pf_part, e->pf_counters, e->stream); }))
         return rc;
     return ok();
+}
+
+// ---- serving over a paged cache ----------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+// Checks of a paged call; *b: its sequences, without work items; *total: its
+// tokens.
+int check_paged(tla_engine* e, const tla_paged_cache* c, int n_seq, const int* pos_host, const int* n_tok_host,
+                int layer, int flags, PagedPool* pool, PagedBatch* b, int* total)
+{
+    if (int rc = check_engine(e)) return rc;
+    if (!c || !pos_host) return fail(TLA_ERR_INVALID_ARGUMENT, "cache and pos must not be NULL");
+    if (n_seq < 1 || n_seq > kMaxSeqPerLaunch)
+        return fail(TLA_ERR_INVALID_ARGUMENT, "n_seq %d not in [1, %d]", n_seq, kMaxSeqPerLaunch);
+    if (flags & ~TLA_ROTATE) return fail(TLA_ERR_INVALID_ARGUMENT, "unknown flags 0x%x", flags);
+    if (layer < 0 || layer >= e->cfg.n_layers)
+        return fail(TLA_ERR_OUT_OF_RANGE, "layer %d outside [0, %d)", layer, e->cfg.n_layers);
+    if (!c->key_pages || !c->value_pages || !c->table_dev)
+        return fail(TLA_ERR_INVALID_ARGUMENT, "NULL device pointer in the cache");
+    if (c->type != TLA_KV_F32 && c->type != TLA_KV_F16 && c->type != TLA_KV_BF16)
+        return fail(TLA_ERR_INVALID_ARGUMENT, "cache type %d", c->type);
+    if (c->page_size < 1 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+        return fail(TLA_ERR_UNSUPPORTED, "page_size %d: powers of two up to 1024 are supported", c->page_size);
+    if (c->n_pages < 1 || c->table_stride < 1)
+        return fail(TLA_ERR_INVALID_ARGUMENT, "n_pages %d, table_stride %d must be >= 1", c->n_pages, c->table_stride);
+    const long long page = static_cast<long long>(c->page_size) * e->kv_dim;
+    const int bytes = c->type == TLA_KV_F32 ? 4 : 2;
+    if (page * bytes >= 1ll << 31) return fail(TLA_ERR_UNSUPPORTED, "a page of %lld elements is 2 GiB or more", page);
+    const size_t page_stride = c->page_stride ? c->page_stride : static_cast<size_t>(page);
+    // so that no product below overflows
+    if (page_stride > size_t(1) << 40 || c->layer_stride > size_t(1) << 50)
+        return fail(TLA_ERR_INVALID_ARGUMENT, "page_stride %zu, layer_stride %zu", page_stride, c->layer_stride);
+    const size_t layer_stride = c->layer_stride ? c->layer_stride : page_stride * c->n_pages;
+    if (page_stride < static_cast<size_t>(page) || page_stride % 8 || layer_stride % 8)
+        return fail(TLA_ERR_INVALID_ARGUMENT, "page_stride %zu, layer_stride %zu: multiples of 8, pages of %lld elements",
+                    page_stride, layer_stride, page);
+    if (!aligned16(c->key_pages) || !aligned16(c->value_pages))
+        return fail(TLA_ERR_INVALID_ARGUMENT, "pages must be 16-byte aligned");
+    const long long held = static_cast<long long>(c->table_stride) * c->page_size;
+    long long t = 0;
+    for (int s = 0; s < n_seq; ++s) {
+        const int n = n_tok_host ? n_tok_host[s] : 1;
+        if (n < 0) return fail(TLA_ERR_INVALID_ARGUMENT, "n_tok[%d] = %d < 0", s, n);
+        const long long end = static_cast<long long>(pos_host[s]) + n;
+        if (pos_host[s] < 0 || end > e->cfg.n_ctx || end > held)
+            return fail(TLA_ERR_OUT_OF_RANGE, "positions [%d, %lld) of sequence %d outside [0, n_ctx=%d) or the table's %lld",
+                        pos_host[s], end, s, e->cfg.n_ctx, held);
+        b->pos[s] = pos_host[s];
+        b->tok[s] = static_cast<int>(t);
+        b->set_id(s, s);
+        t += n;
+        if (t > 1 << 24) return fail(TLA_ERR_UNSUPPORTED, "more than 2^24 tokens");
+    }
+    b->tok[n_seq] = *total = static_cast<int>(t);
+    const size_t off = layer_stride * layer * bytes;
+    pool->k = static_cast<char*>(c->key_pages) + off;
+    pool->v = static_cast<char*>(c->value_pages) + off;
+    pool->table = c->table_dev;
+    pool->page_stride = static_cast<long long>(page_stride);
+    pool->table_stride = c->table_stride;
+    pool->n_pages = c->n_pages;
+    pool->page_shift = __builtin_ctz(c->page_size);
+    pool->type = c->type;
+    return TLA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tla_paged_cache_alloc(tla_engine* e, int n_pages, int page_size, int type, tla_paged_cache* cache)
+{
+    if (int rc = check_engine(e)) return rc;
+    if (!cache) return fail(TLA_ERR_INVALID_ARGUMENT, "cache is NULL");
+    *cache = tla_paged_cache{};
+    if (n_pages < 1) return fail(TLA_ERR_INVALID_ARGUMENT, "n_pages %d < 1", n_pages);
+    if (page_size < 1 || page_size > 1024 || (page_size & (page_size - 1)))
+        return fail(TLA_ERR_UNSUPPORTED, "page_size %d: powers of two up to 1024 are supported", page_size);
+    if (type != TLA_KV_F32 && type != TLA_KV_F16 && type != TLA_KV_BF16)
+        return fail(TLA_ERR_INVALID_ARGUMENT, "cache type %d", type);
+    tla_paged_cache c{};
+    c.type = type;
+    c.page_size = page_size;
+    c.n_pages = n_pages;
+    c.page_stride = static_cast<size_t>(page_size) * e->kv_dim;
+    c.layer_stride = c.page_stride * n_pages;
+    const size_t bytes = c.layer_stride * e->cfg.n_layers * (type == TLA_KV_F32 ? 4 : 2);
+    if (int rc = tla_alloc(e, bytes, &c.key_pages)) return rc;
+    if (int rc = tla_alloc(e, bytes, &c.value_pages)) {
+        tla_free(e, c.key_pages);
+        return rc;
+    }
+    *cache = c;
+    return ok();
+}
+
+int tla_paged_append(tla_engine* e, const tla_paged_cache* cache, int n_seq, const int* pos_host,
+                     const int* n_tok_host, int layer, int flags, const float* k_dev, const float* v_dev)
+{
+    PagedAppendParams p{};
+    PagedBatch b{};
+    int total = 0;
+    if (int rc = check_paged(e, cache, n_seq, pos_host, n_tok_host, layer, flags, &p.pool, &b, &total)) return rc;
+    if (!k_dev || !v_dev) return fail(TLA_ERR_INVALID_ARGUMENT, "NULL device pointer");
+    if (!aligned16(k_dev) || !aligned16(v_dev))
+        return fail(TLA_ERR_INVALID_ARGUMENT, "k and v must be 16-byte aligned");
+    if (total == 0) return ok();
+    if (int rc = set_device(e)) return rc;
+    std::memcpy(b.first, b.tok, sizeof b.first);  // an item is a token
+    p.k = k_dev;
+    p.v = v_dev;
+    p.rope = e->rope;
+    p.n_seq = n_seq;
+    p.n_head_kv = e->cfg.n_head_kv;
+    p.n_items = total;
+    p.rotate = (flags & TLA_ROTATE) ? 1 : 0;
+    return launch(e, TLA_KERNEL_APPEND, "paged append", [&] { return launch_paged_append(p, b, e->stream); });
+}
+
+int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, const int* pos_host,
+                        const int* n_tok_host, int layer, int flags, float* out_dev, const float* q_dev)
+{
+    PagedAttentionParams p{};
+    PagedBatch b{};
+    int total = 0;
+    if (int rc = check_paged(e, cache, n_seq, pos_host, n_tok_host, layer, flags, &p.pool, &b, &total)) return rc;
+    if (!out_dev || !q_dev) return fail(TLA_ERR_INVALID_ARGUMENT, "NULL device pointer");
+    if (!aligned16(out_dev) || !aligned16(q_dev))
+        return fail(TLA_ERR_INVALID_ARGUMENT, "q and the output must be 16-byte aligned");
+    if (total == 0) return ok();
+    if (int rc = set_device(e)) return rc;
+    for (int s = 0; s <= n_seq; ++s) b.first[s] = b.tok[s] * e->cfg.n_head;  // an item is a row of q
+    p.q = q_dev;
+    p.out = out_dev;
+    p.rope = e->rope;
+    p.n_seq = n_seq;
+    p.n_head = e->cfg.n_head;
+    p.n_head_kv = e->cfg.n_head_kv;
+    p.gqa = e->gqa;
+    p.n_items = total * e->cfg.n_head;
+    p.rotate = (flags & TLA_ROTATE) ? 1 : 0;
+    p.scale_log2 = scale_log2(e->head_dim);
+    return launch(e, TLA_KERNEL_PREFILL, "paged attention", [&] { return launch_paged_attention(p, b, e->stream); });
+}
+
+int tla_logits_process(tla_engine* e, int n_seq, int n_vocab, const tla_logit_rules* rules, float* out_dev,
+                       const float* logits_dev, int* tokens_dev)
+{
+    if (int rc = check_engine(e)) return rc;
+    if (!out_dev || !logits_dev) return fail(TLA_ERR_INVALID_ARGUMENT, "NULL device pointer");
+    if (n_seq < 1 || n_vocab < 1) return fail(TLA_ERR_INVALID_ARGUMENT, "n_seq %d, n_vocab %d must be >= 1", n_seq, n_vocab);
+    if (n_seq > 1 << 16 || n_vocab > 1 << 28)
+        return fail(TLA_ERR_UNSUPPORTED, "n_seq %d > 2^16 or n_vocab %d > 2^28", n_seq, n_vocab);
+    LogitsParams p{};
+    if (rules) {
+        p.rules = *rules;
+        const tla_logit_rules& r = *rules;
+        if (r.history_dev && (!r.history_len_dev || !r.penalties_dev || r.history_stride < 1))
+            return fail(TLA_ERR_INVALID_ARGUMENT, "a history needs its lengths, penalties and a stride >= 1");
+        if (r.bias_token_dev && (!r.bias_value_dev || !r.bias_len_dev || r.bias_stride < 1))
+            return fail(TLA_ERR_INVALID_ARGUMENT, "biases need their values, lengths and a stride >= 1");
+        if (r.mask_dev && r.mask_stride < (n_vocab + 31) / 32)
+            return fail(TLA_ERR_INVALID_ARGUMENT, "mask_stride %d < ceil(n_vocab / 32)", r.mask_stride);
+    }
+    if (int rc = set_device(e)) return rc;
+    p.x = logits_dev;
+    p.out = out_dev;
+    p.tokens = tokens_dev;
+    p.n_vocab = n_vocab;
+    p.n_slices = logits_slices(n_vocab);
+    if (static_cast<long long>(n_seq) * p.n_slices > 0x7fffffff)
+        return fail(TLA_ERR_UNSUPPORTED, "%d rows of %d logits", n_seq, n_vocab);
+    if (tokens_dev) {
+        if (int rc = ensure_buf(e, reinterpret_cast<void**>(&e->best), e->best_bytes,
+                                sizeof(unsigned long long) * n_seq * p.n_slices, "logits' best tokens"))
+            return rc;
+        if (int rc = ensure_counters(e, &e->best_counters, e->n_best_counters, n_seq)) return rc;
+        p.best = e->best;
+        p.counters = e->best_counters;
+    }
+    return launch(e, TLA_KERNEL_LOGITS, "logits", [&] { return launch_logits_process(p, n_seq, e->stream); });
 }
 
 // ---- FFN, embedding, sampling, the whole forward pass ------------------------

@@ -1,0 +1,26 @@
+// Rules on a batch of logits: launches of logits.hip.
+#pragma once
+
+#include "tla_internal.h"
+
+namespace tla {
+
+struct LogitsParams {
+    const float* x;  // [n_seq][n_vocab]
+    float* out;      // may be x
+    int* tokens;     // [n_seq], or NULL
+    int n_vocab;
+    int n_slices;    // workgroups per row
+    tla_logit_rules rules;
+    // With tokens: each workgroup's best (an argmax key), [n_seq][n_slices],
+    // and the rows' arrivals, zero between launches.
+    unsigned long long* best;
+    int* counters;
+};
+
+// Workgroups per row of n_vocab logits.
+int logits_slices(int n_vocab);
+hipError_t launch_logits_process(const LogitsParams& p, int n_seq, hipStream_t s);
+hipError_t load_logits_code();
+
+}  // namespace tla

@@ -1,0 +1,77 @@
+// Paged KV cache: launches of paged.hip.
+#pragma once
+
+#include "tla_internal.h"
+
+namespace tla {
+
+enum KvType { kKvF32 = 0, kKvF16 = 1, kKvBF16 = 30 };  // the ggml_type ids of the elements
+
+// One layer of a paged cache.  Position p of sequence s is row p % page_size
+// of page table[s * table_stride + p / page_size]; an entry outside
+// [0, n_pages) is an absent page: nothing is written to it, and its positions
+// are not attended to.
+struct PagedPool {
+    void* k;               // page 0 of the layer
+    void* v;
+    const int* table;
+    long long page_stride;  // elements
+    int table_stride;
+    int n_pages;
+    int page_shift;        // page_size = 1 << page_shift
+    int type;              // KvType
+};
+
+// The sequences of one launch, in the kernel arguments: sequence s holds
+// pos[s] positions before the call, its new tokens are rows tok[s] ..
+// tok[s + 1] - 1 of the packed inputs.  Work items are handed out by rank:
+// rank r is sequence id(r), its items first[r] .. first[r + 1] - 1 (none for a
+// sequence that this launch does not serve).  The ids are bytes of whole words:
+// from an array of bytes next to arrays of words the compiler made scalar word
+// loads whose base address is not a multiple of 4, which the hardware rounds
+// down (ROCm 7.2).
+template <int kMaxSeq>
+struct PagedSeqs {
+    int pos[kMaxSeq];
+    int tok[kMaxSeq + 1];
+    int first[kMaxSeq + 1];
+    unsigned ids[kMaxSeq / 4];
+    __host__ __device__ int id(int rank) const { return (int)(ids[rank >> 2] >> (8 * (rank & 3)) & 255); }
+    void set_id(int rank, int s)
+    {
+        ids[rank >> 2] = (ids[rank >> 2] & ~(255u << (8 * (rank & 3)))) | (unsigned)s << (8 * (rank & 3));
+    }
+};
+static_assert(kMaxSeqPerLaunch <= 256, "PagedSeqs::ids");
+typedef PagedSeqs<kMaxSeqPerLaunch> PagedBatch;
+
+struct PagedAppendParams {
+    PagedPool pool;
+    const float* k;  // [total tokens][n_head_kv][64]
+    const float* v;
+    const float2* rope;
+    int n_seq;
+    int n_head_kv;
+    int n_items;
+    int rotate;
+};
+hipError_t launch_paged_append(const PagedAppendParams& p, const PagedBatch& b, hipStream_t s);
+
+struct PagedAttentionParams {
+    PagedPool pool;
+    const float* q;  // [total tokens][n_head][64]
+    float* out;
+    const float2* rope;
+    int n_seq;
+    int n_head;
+    int n_head_kv;
+    int gqa;
+    int n_items;
+    int rotate;
+    float scale_log2;
+};
+hipError_t launch_paged_attention(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s);
+
+hipError_t load_paged_code();
+
+}  // namespace tla
