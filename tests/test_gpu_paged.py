@@ -194,6 +194,25 @@ def test_output_in_place_of_the_queries(O, engines):
             assert np.all(np.abs(a["q"].download() - want) <= bound)
 
 
+@pytest.mark.parametrize("n_tok", [1, 40])
+def test_output_in_place_of_the_queries_with_infinite_values(O, engines, n_tok):
+    """Rows that are computed once more read their queries once more."""
+    eng = engines(1, 2048)
+    b = Batch(38, eng.cfg, F16, 16, [60], [n_tok])
+    b.append(O)
+    want, bound = b.attend(O)
+    page, at = b.table[0, 0], 3 * b.kv + 64 + 5
+    b.vp[0, page, at] = to_bits(np.array([np.inf]), F16)[0]
+    with b.on(eng) as (cache, a):
+        eng.paged_attention(cache, b.pos, b.n_tok, 0, a["q"].ptr, a["q"].ptr)
+        got = a["q"].download()
+    hit = np.zeros((n_tok, 32, 64), bool)
+    hit[:, 8:16, 5] = True
+    hit = hit.reshape(n_tok, -1)
+    assert np.all(got[hit] == np.inf)
+    assert np.all(np.abs(got - want)[~hit] <= bound[~hit])
+
+
 def test_sequences_that_share_pages(O, engines):
     """Two sequences with a prefix in common, each with tokens of its own."""
     eng = engines(1, 2048)

@@ -1399,15 +1399,15 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
                         const int* n_tok_host, int layer, int flags, float* out_dev, const float* q_dev)
 {
     PagedAttentionParams p{};
-    PagedBatch b{};
+    PagedPlan plan{};
     int total = 0;
-    if (int rc = check_paged(e, cache, n_seq, pos_host, n_tok_host, layer, flags, &p.pool, &b, &total)) return rc;
+    if (int rc = check_paged(e, cache, n_seq, pos_host, n_tok_host, layer, flags, &p.pool, &plan.batch, &total))
+        return rc;
     if (!out_dev || !q_dev) return fail(TLA_ERR_INVALID_ARGUMENT, "NULL device pointer");
     if (!aligned16(out_dev) || !aligned16(q_dev))
         return fail(TLA_ERR_INVALID_ARGUMENT, "q and the output must be 16-byte aligned");
     if (total == 0) return ok();
     if (int rc = set_device(e)) return rc;
-    for (int s = 0; s <= n_seq; ++s) b.first[s] = b.tok[s] * e->cfg.n_head;  // an item is a row of q
     p.q = q_dev;
     p.out = out_dev;
     p.rope = e->rope;
@@ -1415,10 +1415,29 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
     p.n_head = e->cfg.n_head;
     p.n_head_kv = e->cfg.n_head_kv;
     p.gqa = e->gqa;
-    p.n_items = total * e->cfg.n_head;
     p.rotate = (flags & TLA_ROTATE) ? 1 : 0;
     p.scale_log2 = scale_log2(e->head_dim);
-    return launch(e, TLA_KERNEL_PREFILL, "paged attention", [&] { return launch_paged_attention(p, b, e->stream); });
+    for (const bool chunk : {true, false}) {
+        if (chunk)
+            plan_chunk(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &plan);
+        else
+            plan_stream(n_seq, p.n_head_kv, p.gqa, e->n_cu, &plan);
+        if (plan.n_items == 0) continue;
+        if (plan.shared) {
+            const size_t items = static_cast<size_t>(plan.n_items);
+            if (int rc = ensure_ws(e, items * (chunk ? kChunkStateBytes : kStreamStateBytes))) return rc;
+            if (int rc = ensure_counters(e, &e->counters, e->n_counters, items)) return rc;
+            p.part = static_cast<float*>(e->ws);
+            p.counters = e->counters;
+        }
+        p.n_items = plan.n_items;
+        p.split_tiles = plan.split_tiles;
+        if (int rc = launch(e, chunk ? TLA_KERNEL_PREFILL : TLA_KERNEL_DECODE, "paged attention", [&] {
+                return chunk ? launch_paged_chunk(p, plan.batch, e->stream) : launch_paged_stream(p, plan.batch, e->stream);
+            }))
+            return rc;
+    }
+    return ok();
 }
 
 int tla_logits_process(tla_engine* e, int n_seq, int n_vocab, const tla_logit_rules* rules, float* out_dev,

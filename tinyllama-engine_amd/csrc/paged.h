@@ -62,15 +62,39 @@ struct PagedAttentionParams {
     const float* q;  // [total tokens][n_head][64]
     float* out;
     const float2* rope;
+    float* part;     // softmax states of workgroups that share rows, by work item
+    int* counters;   // and their arrivals, by the rows' first work item; zero between launches
     int n_seq;
     int n_head;
     int n_head_kv;
     int gqa;
     int n_items;
+    int split_tiles; // key tiles per work item at most
     int rotate;
     float scale_log2;
 };
-hipError_t launch_paged_attention(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s);
+
+// How one call's sequences are served: those of at most kStreamRows query rows
+// per kv head stream their keys and values past rows held in registers
+// (paged_stream_kernel), longer chunks go through LDS tiles
+// (paged_chunk_kernel).
+constexpr int kStreamRows = 16;
+constexpr int kStreamTile = 32;  // keys per tile of one wave
+constexpr int kChunkRows = 128;  // query rows of a workgroup
+struct PagedPlan {
+    PagedBatch batch;  // pos and tok set by the caller
+    int n_items;       // 0: no such sequence in the call
+    int split_tiles;
+    bool shared;       // some rows are shared by several work items
+};
+// Bytes of one work item's softmax state.
+constexpr int kStreamStateBytes = 64 * 18 * 4;
+constexpr int kChunkStateBytes = 4 * 64 * 34 * 4;
+int chunk_tile(int type);  // keys per tile of paged_chunk_kernel
+void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, PagedPlan* p);
+void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* p);
+hipError_t launch_paged_stream(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s);
+hipError_t launch_paged_chunk(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s);
 
 hipError_t load_paged_code();
 

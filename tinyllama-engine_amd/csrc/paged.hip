@@ -1,5 +1,9 @@
 // Paged KV cache for gfx950: append of new keys (rotated) and values, and
 // attention of new tokens over their sequences' pages.
+#include <algorithm>
+
+#include "bf16_split.h"
+#include "lane_math.h"
 #include "paged.h"
 #include "rope_math.h"
 
@@ -166,20 +170,839 @@ __device__ __forceinline__ float q_lane(const float* q, const float2* cs, int ro
     return x * scale;
 }
 
-// One wave per (token, head).
-template <int kType, int kMaxSeq>
-__global__ __launch_bounds__(256) void paged_attention_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kRawBufferWord3 = 0x00020000;  // untyped 32-bit buffer (gfx9 family)
+constexpr int kDeviceScope = 16;             // cache-policy bit SC1: device scope
+constexpr float kRescaleSlack = 8.f;         // log2 units a running max may lag behind
+
+// Products with fp32 accuracy on the 16-bit matrix cores.  A key or value of
+// the cache is exact in its own type; an fp32 operand (a query, a
+// probability) is a sum of pieces of that type, and every product of two
+// 16-bit numbers is exact in the fp32 accumulator.
+//   F16: two pieces, 22 bits: to 2^-22 of the operand, or to 2^-25 (half the
+//   smallest step of an F16) where that is more.  Query rows are brought to
+//   2^13 .. 2^14 by a power of two first, probabilities carry a factor of 2^6,
+//   so that the latter is below 2^-38 of the row's largest.
+//   BF16: three pieces, all 24 bits, in fp32's own range.
+//   F32: the cache's elements are three BF16 pieces as well: the six products of
+//   pieces down to 2^-16 (the three left out are below 2^-24).
+template <int kType>
+struct Pieces;
+template <>
+struct Pieces<kKvF16> {
+    typedef f16x8 Frag;
+    static constexpr int kN = 2;
+    static constexpr float kShift = 6.f;
+    static constexpr bool kScaled = true;
+    static __device__ __forceinline__ void split(floatx8 v, Frag (&o)[kN])
+    {
+        o[0] = __builtin_convertvector(v, f16x8);
+        o[1] = __builtin_convertvector(v - __builtin_convertvector(o[0], floatx8), f16x8);
+    }
+    static __device__ __forceinline__ floatx4 mfma16(Frag a, Frag b, floatx4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ floatx16 mfma32(Frag a, Frag b, floatx16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Pieces<kKvBF16> {
+    typedef bf16x8 Frag;
+    static constexpr int kN = 3;
+    static constexpr float kShift = 0.f;
+    static constexpr bool kScaled = false;
+    static __device__ __forceinline__ void split(floatx8 v, Frag (&o)[kN]) { split3x8(v, o[0], o[1], o[2]); }
+    static __device__ __forceinline__ floatx4 mfma16(Frag a, Frag b, floatx4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ floatx16 mfma32(Frag a, Frag b, floatx16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Pieces<kKvF32> : Pieces<kKvBF16> {};
+
+// The power of two that brings a row whose largest magnitude is `top` to
+// 2^13 .. 2^14, and its inverse.  Rows of zeros, and of numbers so small or
+// large that the factor would leave the fp32 range, get the nearest one that
+// does not.
+__device__ __forceinline__ void row_scale(float top, float& up, float& down)
 {
-    const int item = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    if (item >= p.n_items) return;
-    const int lane = threadIdx.x & (kWave - 1);
-    const int rank = rank_of(b, p.n_seq, item), i = b.id(rank);
-    const int t = (item - b.first[rank]) / p.n_head, h = (item - b.first[rank]) % p.n_head;
-    const int qpos = b.pos[i] + t;
-    const long long row = ((long long)(b.tok[i] + t) * p.n_head + h) * kHeadDim;
-    const float x = q_lane(p.q + row, p.rope + (long long)qpos * kPairs, p.rotate, p.scale_log2);
-    p.out[row + lane] = plain_row<kType>(p.pool, p.pool.table + (long long)i * p.pool.table_stride,
-                                         p.n_head_kv * kHeadDim, h / p.gqa * kHeadDim, qpos, x);
+    const int e = (int)(__builtin_bit_cast(unsigned, top) >> 23 & 255) - 127;
+    const int s = min(max(13 - e, -100), 100);
+    up = __builtin_bit_cast(float, (unsigned)(127 + s) << 23);
+    down = __builtin_bit_cast(float, (unsigned)(127 - s) << 23);
+}
+
+// The rotation of rotate4 with fused multiply-adds, for operands that are not
+// stored (q).
+__device__ __forceinline__ float4 rotate4_fma(float4 x, float4 cs)
+{
+    return make_float4(__builtin_fmaf(x.x, cs.x, -(x.y * cs.y)), __builtin_fmaf(x.x, cs.y, x.y * cs.x),
+                       __builtin_fmaf(x.z, cs.z, -(x.w * cs.w)), __builtin_fmaf(x.z, cs.w, x.w * cs.z));
+}
+
+__device__ __forceinline__ floatx4 scaled_q4(const float* q, const float* cs, int d, int rotate, float scale)
+{
+    float4 x = ldg4(q + d);
+    x = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
+    if (rotate) x = rotate4_fma(x, ldg4(cs + d));
+    return floatx4{x.x, x.y, x.z, x.w};
+}
+
+__device__ __forceinline__ bool not_finite(float x)
+{
+    return !(__builtin_fabsf(x) <= 3.4028234663852886e38f);
+}
+
+// Up to 16 rows of 64 elements of one kv head from one page, as a buffer
+// whose range ends with them: loads past the last row, and all of an absent
+// page's, give zeros without touching memory.
+struct Rows {
+    const char* base;
+    unsigned bytes;  // 0: absent
+};
+__device__ __forceinline__ auto rsrc_of(const Rows& r)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(r.base), 0, r.bytes, kRawBufferWord3);
+}
+
+// Counts this workgroup in after its device-scope stores are acknowledged;
+// true for the last of n, which also returns the counter to zero.  All
+// threads of the workgroup call it.
+__device__ __forceinline__ bool last_to_arrive(int* counter, int n, int& s_last)
+{
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0)
+        s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+    __syncthreads();
+    const bool last = s_last;
+    if (last && threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return last;
+}
+
+// A wave's operands of one 32-key tile, as the 16x16 MFMAs read them, and the
+// two products.  Lane l = 16 g + c.  Keys: K operand row c of half hf is key
+// 16 hf + c, so that score register r of lane (g, c) is key 16 hf + 4 g + r
+// for query row c.  The same registers are the B operand (P^T) of the P.V
+// product if V's k index 8 g + e is key 4 g + e (e < 4) or 16 + 4 g + e - 4.
+// V operand row c of dt holds dimension 4 c + dt, so that O register r of dt
+// is dimension 16 g + 4 r + dt of query row c.
+template <int kType>
+struct StreamTile {
+    typedef Pieces<kType> P;
+    typedef typename P::Frag Frag;
+    // k step ks: dimensions 16 g + 8 ks .. + 7
+    uintx4 k[2][2];
+    uintx2 v[8];
+    struct Query {
+        Frag f[2][P::kN];
+        float down;
+    };
+    static constexpr int kKeyBytes = 16;
+    template <class L>
+    __device__ __forceinline__ void load_k(int hf, L&& load16)
+    {
+        k[hf][0] = load16(0);
+        k[hf][1] = load16(16);
+    }
+    template <class L>
+    __device__ __forceinline__ void load_v(int hf, int r, L&& load8)
+    {
+        v[4 * hf + r] = load8();
+    }
+    // x: dimensions 16 g .. + 15 of the row
+    static __device__ __forceinline__ void query(const floatx4 (&x)[4], Query& q)
+    {
+        float up = 1.f;
+        q.down = 1.f;
+        if constexpr (P::kScaled) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, __builtin_fabsf(x[i][e]));
+            row_scale(max_xor32(max_xor16(top)), up, q.down);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            floatx8 v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = x[2 * ks + (e >> 2)][e & 3] * up;
+            P::split(v, q.f[ks]);
+        }
+    }
+    __device__ __forceinline__ floatx4 scores(int hf, const Query& q) const
+    {
+        floatx4 s = {};
+#pragma unroll
+        for (int i = P::kN - 1; i >= 0; --i)  // small ones first
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) s = P::mfma16(__builtin_bit_cast(Frag, k[hf][ks]), q.f[ks][i], s);
+        return s;
+    }
+    __device__ __forceinline__ void accumulate(const floatx4 (&p)[2], floatx4 (&o)[4]) const
+    {
+        Frag f[P::kN];
+        P::split(floatx8{p[0][0], p[0][1], p[0][2], p[0][3], p[1][0], p[1][1], p[1][2], p[1][3]}, f);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) {
+            uintx4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[i] = __builtin_amdgcn_perm(v[2 * i + 1][dt >> 1], v[2 * i][dt >> 1], dt & 1 ? 0x07060302 : 0x05040100);
+            const Frag a = __builtin_bit_cast(Frag, w);
+#pragma unroll
+            for (int i = P::kN - 1; i >= 0; --i) o[dt] = P::mfma16(a, f[i], o[dt]);
+        }
+    }
+};
+// fp32 elements: the fp32 MFMA, exact products at the rate that one pass over
+// the keys needs.  Its 16 k steps take dimensions 16 g + i.
+template <>
+struct StreamTile<kKvF32> {
+    floatx4 k[2][4];
+    floatx4 v[8];
+    struct Query {
+        floatx4 x[4];
+        float down;
+    };
+    static constexpr int kKeyBytes = 32;
+    template <class L>
+    __device__ __forceinline__ void load_k(int hf, L&& load16)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[hf][i] = __builtin_bit_cast(floatx4, load16(16 * i));
+    }
+    template <class L>
+    __device__ __forceinline__ void load_v(int hf, int r, L&& load16)
+    {
+        v[4 * hf + r] = __builtin_bit_cast(floatx4, load16());
+    }
+    static __device__ __forceinline__ void query(const floatx4 (&x)[4], Query& q)
+    {
+        q.down = 1.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q.x[i] = x[i];
+    }
+    __device__ __forceinline__ floatx4 scores(int hf, const Query& q) const
+    {
+        floatx4 s = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[hf][i][e], q.x[i][e], s, 0, 0, 0);
+        return s;
+    }
+    __device__ __forceinline__ void accumulate(const floatx4 (&p)[2], floatx4 (&o)[4]) const
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j][dt], p[j >> 2][j & 3], o[dt], 0, 0, 0);
+    }
+};
+
+// Rows of one sequence and kv head: up to 16 (token, head) pairs, row c being
+// token c / gqa, head c % gqa of the kv head.  One work item is a range of
+// split_tiles 32-key tiles, its four waves taking every fourth tile each, with
+// no word to each other until the end: then the waves' states meet in LDS,
+// and the items of one unit in the workspace, where the last to arrive adds
+// them in order.
+// kSmall: pages of fewer than 16 positions, whose rows are looked up one by
+// one; else each half of a tile lies in one page, looked up by the wave.
+template <int kType, bool kSmall, int kMaxSeq>
+__global__ __launch_bounds__(256) void paged_stream_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
+{
+    typedef typename Elem<kType>::T T;
+    typedef StreamTile<kType> Tile;
+    __shared__ floatx4 s_o[4][4][kWave];  // [wave][r][lane]
+    __shared__ float2 s_ml[4][kWave];
+    __shared__ int s_bad[16];
+    __shared__ int s_last;
+    const int item = blockIdx.x;
+    const int rank = rank_of(b, p.n_seq, item), seq = b.id(rank);
+    const int local = item - b.first[rank];
+    const int kvh = local % p.n_head_kv, split = local / p.n_head_kv;
+    const int n_split = (b.first[rank + 1] - b.first[rank]) / p.n_head_kv;
+    const int pos = b.pos[seq], n_tok = b.tok[seq + 1] - b.tok[seq];
+    const int len = pos + n_tok, n_rows = n_tok * p.gqa;
+    const int n_tiles = (len + kStreamTile - 1) / kStreamTile;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kWave - 1);
+    const int c = lane & 15, g = lane >> 4;
+    const int* const table = p.pool.table + (long long)seq * p.pool.table_stride;
+    const int kv_dim = p.n_head_kv * kHeadDim, head_off = kvh * kHeadDim;
+
+    // The row's query.  Rows past the last repeat it (their results are not stored).
+    const int row = min(c, n_rows - 1), t = row / p.gqa, qpos = pos + t;
+    const long long q_at = ((long long)(b.tok[seq] + t) * p.n_head + kvh * p.gqa + row - t * p.gqa) * kHeadDim;
+    const float* const cs = reinterpret_cast<const float*>(p.rope + (long long)qpos * kPairs);
+    if (threadIdx.x < 16) s_bad[threadIdx.x] = 0;
+
+    Tile cur, next;
+    bool cur_seen[2], next_seen[2];        // kSmall: none; the halves' pages are there
+    unsigned cur_mask = 0, next_mask = 0;  // kSmall: bit 4 hf + r, the row is there
+    const auto look_up = [&](int tile, int (&page)[2]) {
+        if constexpr (!kSmall) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) page[hf] = table[min(tile * kStreamTile + 16 * hf, len - 1) >> p.pool.page_shift];
+        }
+    };
+    const auto load = [&](int tile, const int (&page)[2], Tile& d, bool (&seen)[2], unsigned& mask) {
+        if constexpr (kSmall) {
+            mask = 0;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int kk = tile * kStreamTile + 16 * hf + c;
+                const long long kr = kk < len ? row_of(p.pool, table, kk, kv_dim) : -1;
+                const char* const ka = reinterpret_cast<const char*>(static_cast<const T*>(p.pool.k) + kr + head_off) + Tile::kKeyBytes * 2 * g;
+                d.load_k(hf, [&](int o) { return kr >= 0 ? *reinterpret_cast<const uintx4*>(ka + o) : uintx4{}; });
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int vk = tile * kStreamTile + 16 * hf + 4 * g + r;
+                    const long long vr = vk < len ? row_of(p.pool, table, vk, kv_dim) : -1;
+                    const T* const va = static_cast<const T*>(p.pool.v) + vr + head_off + 4 * c;
+                    typedef std::conditional_t<kType == kKvF32, uintx4, uintx2> V;
+                    d.load_v(hf, r, [&] { return vr >= 0 ? *reinterpret_cast<const V*>(va) : V{}; });
+                    mask |= vr >= 0 ? 1u << (4 * hf + r) : 0u;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int key = tile * kStreamTile + 16 * hf;
+                seen[hf] = key < len && (unsigned)page[hf] < (unsigned)p.pool.n_pages;
+                const long long at = (long long)page[hf] * p.pool.page_stride +
+                                     (long long)(key & ((1 << p.pool.page_shift) - 1)) * kv_dim + head_off;
+                const unsigned row_bytes = kv_dim * sizeof(T);
+                const unsigned bytes = seen[hf] ? (min(16, len - key) - 1) * row_bytes + kHeadDim * (unsigned)sizeof(T) : 0;
+                const auto rk = rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(p.pool.k) + (seen[hf] ? at : 0)), bytes});
+                const auto rv = rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(p.pool.v) + (seen[hf] ? at : 0)), bytes});
+                d.load_k(hf, [&](int o) {
+                    return __builtin_amdgcn_raw_buffer_load_b128(rk, c * row_bytes + Tile::kKeyBytes * 2 * g + o, 0, 0);
+                });
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    d.load_v(hf, r, [&] {
+                        if constexpr (kType == kKvF32)
+                            return __builtin_amdgcn_raw_buffer_load_b128(rv, (4 * g + r) * row_bytes + 16 * c, 0, 0);
+                        else
+                            return __builtin_amdgcn_raw_buffer_load_b64(rv, (4 * g + r) * row_bytes + 8 * c, 0, 0);
+                    });
+            }
+        }
+    };
+
+    int tile = split * p.split_tiles + wave;
+    const int tile_end = min((split + 1) * p.split_tiles, n_tiles);
+    int page[2] = {};
+    if (tile < tile_end) {  // first the keys, on whose way the query is rotated
+        look_up(tile, page);
+        load(tile, page, cur, cur_seen, cur_mask);
+        look_up(min(tile + 4, n_tiles - 1), page);
+    }
+    typename Tile::Query q;
+    {
+        floatx4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = scaled_q4(p.q + q_at, cs, 16 * g + 4 * i, p.rotate, p.scale_log2);
+        Tile::query(x, q);
+    }
+    floatx4 o[4] = {};
+    float m_run = -INFINITY, l_run = 0.f;
+    constexpr float kShift = Pieces<kType>::kShift;
+    for (; tile < tile_end; tile += 4) {
+        if (tile + 4 < tile_end) {
+            load(tile + 4, page, next, next_seen, next_mask);
+            look_up(min(tile + 8, n_tiles - 1), page);
+        }
+        floatx4 s[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) s[hf] = cur.scores(hf, q) * q.down;
+        const int key = tile * kStreamTile + 4 * g;
+        if (kSmall || (tile + 1) * kStreamTile > pos + 1 || !cur_seen[0] || !cur_seen[1]) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool there = kSmall ? (cur_mask >> (4 * hf + r) & 1) != 0 : cur_seen[hf];
+                    s[hf][r] = there && key + 16 * hf + r <= qpos ? s[hf][r] : -INFINITY;
+                }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = max_xor32(max_xor16(mx));
+        // The running max moves only when a row's exceeds it by more than the
+        // slack: most tiles do not rescale O.  A row that has seen nothing
+        // keeps -inf; its probabilities are 0.
+        if (__any(mx > m_run + kRescaleSlack)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
+        }
+        const float m_use = m_run == -INFINITY ? 0.f : m_run - kShift;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[hf][r] = __builtin_amdgcn_exp2f(s[hf][r] - m_use);
+                l_run += s[hf][r];
+            }
+        cur.accumulate(s, o);
+        if (tile + 4 < tile_end) {
+            cur = next;
+            cur_seen[0] = next_seen[0];
+            cur_seen[1] = next_seen[1];
+            cur_mask = next_mask;
+        }
+    }
+    l_run = sum_xor32(sum_xor16(l_run));  // the lane groups summed different keys
+
+    // The four waves' states meet: wave w goes on with dimensions 16 g + 4 w .. + 3.
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s_o[wave][r][lane] = floatx4{o[0][r], o[1][r], o[2][r], o[3][r]};
+    s_ml[wave][lane] = make_float2(m_run, l_run);
+    __syncthreads();
+    floatx4 acc = {};
+    const auto merge = [&](int n, auto&& ml_of, auto&& o_of) {
+        float m_new = -INFINITY;
+        for (int i = 0; i < n; ++i) m_new = fmaxf(m_new, ml_of(i).x);
+        m_run = m_new;
+        l_run = 0.f;
+        acc = floatx4{};
+        for (int i = 0; i < n; ++i) {
+            const float2 ml = ml_of(i);
+            const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m_new);
+            l_run = fmaf(ml.y, f, l_run);
+            acc += o_of(i) * f;
+        }
+    };
+    merge(4, [&](int i) { return s_ml[i][lane]; }, [&](int i) { return s_o[i][wave][lane]; });
+    if (n_split > 1) {
+        const auto part_of = [&](int s) {
+            return __builtin_amdgcn_make_buffer_rsrc(
+                p.part + (long long)(b.first[rank] + s * p.n_head_kv + kvh) * (kStreamStateBytes / 4), 0, kStreamStateBytes,
+                kRawBufferWord3);
+        };
+        const auto mine = part_of(split);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, acc), mine, 1024 * wave + 16 * lane, 0, kDeviceScope);
+        if (wave == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uintx2, make_float2(m_run, l_run)), mine, 4096 + 8 * lane, 0,
+                                                  kDeviceScope);
+        if (!last_to_arrive(p.counters + b.first[rank] + kvh, n_split, s_last)) return;
+        merge(n_split,
+              [&](int i) {
+                  return __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_of(i), 4096 + 8 * lane, 0, kDeviceScope));
+              },
+              [&](int i) {
+                  return __builtin_bit_cast(floatx4,
+                                            __builtin_amdgcn_raw_buffer_load_b128(part_of(i), 1024 * wave + 16 * lane, 0, kDeviceScope));
+              });
+    }
+    const bool real = c < n_rows;
+    const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+    acc *= inv;
+    const bool bad = real && (not_finite(l_run) || not_finite(acc[0]) || not_finite(acc[1]) || not_finite(acc[2]) || not_finite(acc[3]));
+    if (bad) s_bad[c] = 1;
+    __syncthreads();  // the row as a whole: its query may lie where its output goes
+    if (real && !s_bad[c]) stg4(p.out + q_at + 16 * g + 4 * wave, make_float4(acc[0], acc[1], acc[2], acc[3]));
+    // Rows that met something infinite or NaN, seen or not, once more in plain fp32.
+    for (int i = wave; i < n_rows; i += 4) {
+        if (!s_bad[i]) continue;
+        const int ti = i / p.gqa;
+        const long long at = ((long long)(b.tok[seq] + ti) * p.n_head + kvh * p.gqa + i - ti * p.gqa) * kHeadDim;
+        const float x = q_lane(p.q + at, p.rope + (long long)(pos + ti) * kPairs, p.rotate, p.scale_log2);
+        p.out[at + lane] = plain_row<kType>(p.pool, table, kv_dim, head_off, pos + ti, x);
+    }
+}
+
+// ---- chunks --------------------------------------------------------------------------
+
+// A tile's keys and values in LDS, in the order in which the 32x32 MFMA
+// operands are read: planes of 32 keys, one per piece.
+//   K plane: byte 512 c + 16 (kperm(i) ^ c) = dimensions 8 c .. + 7 of key i; kperm
+//     as in the prefill kernel makes the scores of the S accumulator the B
+//     operand of P.V, c spreads the eight pieces of a row that one load
+//     brings over the banks.
+//   V plane: byte 2048 dt + 1024 s + 512 h + 16 i = keys 16 s + 8 h .. + 7 of dimension 2 i + dt.
+constexpr int kPlane = 32 * kHeadDim * 2;
+
+__device__ __forceinline__ int kperm(int i)
+{
+    return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1);
+}
+
+template <int kType>
+struct ChunkTile {
+    typedef Pieces<kType> P;
+    typedef typename P::Frag Frag;
+    static constexpr int kCache = kType == kKvF32 ? 3 : 1;  // planes of a cache element
+    static constexpr int kSub = kType == kKvF32 ? 1 : 2;    // 32-key planes per tile
+    static constexpr int kKeys = 32 * kSub;
+    static constexpr int kBytes = 2 * kCache * kPlane;      // K and V planes of 32 keys
+    typedef std::conditional_t<kType == kKvF32, floatx8, uintx4> KRaw;                          // 8 dimensions of a key
+    typedef std::conditional_t<kType == kKvF32, floatx2, unsigned> VRaw;                        // 2 dimensions of a key
+
+    // One thread's share of 32 keys: dimensions 8 kc .. of key kk, dimensions
+    // 2 vi, 2 vi + 1 of keys 4 vg ..
+    static __device__ __forceinline__ void store(const KRaw& k, const VRaw (&v)[4], unsigned char* at, int kk, int kc,
+                                                 int vi, int vg)
+    {
+        const int k_at = 512 * kc + 16 * (kperm(kk) ^ kc);
+        const int v_at = 1024 * (vg >> 2) + 512 * (vg >> 1 & 1) + 16 * vi + 8 * (vg & 1);
+        if constexpr (kType == kKvF32) {
+            Frag f[3];
+            P::split(k, f);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) *reinterpret_cast<Frag*>(at + i * kPlane + k_at) = f[i];
+            floatx8 x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = v[e & 3][e >> 2];
+            P::split(x, f);  // dt 0, then dt 1
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const uintx4 w = __builtin_bit_cast(uintx4, f[i]);
+                unsigned char* const va = at + (3 + i) * kPlane + v_at;
+                *reinterpret_cast<uintx2*>(va) = uintx2{w[0], w[1]};
+                *reinterpret_cast<uintx2*>(va + 2048) = uintx2{w[2], w[3]};
+            }
+        } else {
+            *reinterpret_cast<uintx4*>(at + k_at) = k;
+            unsigned char* const va = at + kPlane + v_at;
+            *reinterpret_cast<uintx2*>(va) = uintx2{__builtin_amdgcn_perm(v[1], v[0], 0x05040100), __builtin_amdgcn_perm(v[3], v[2], 0x05040100)};
+            *reinterpret_cast<uintx2*>(va + 2048) = uintx2{__builtin_amdgcn_perm(v[1], v[0], 0x07060302), __builtin_amdgcn_perm(v[3], v[2], 0x07060302)};
+        }
+    }
+    static __device__ __forceinline__ floatx16 products(const Frag (&a)[kCache], const Frag (&b)[P::kN], floatx16 c)
+    {
+        if constexpr (kType == kKvF32) {
+            c = P::mfma32(a[2], b[0], c);
+            c = P::mfma32(a[1], b[1], c);
+            c = P::mfma32(a[0], b[2], c);
+            c = P::mfma32(a[1], b[0], c);
+            c = P::mfma32(a[0], b[1], c);
+            c = P::mfma32(a[0], b[0], c);
+        } else {
+#pragma unroll
+            for (int i = P::kN - 1; i >= 0; --i) c = P::mfma32(a[0], b[i], c);
+        }
+        return c;
+    }
+    static __device__ __forceinline__ floatx16 scores(const unsigned char* at, const Frag (&q)[4][P::kN], int lane)
+    {
+        floatx16 s = {};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const int c = 2 * ks + (lane >> 5);
+            Frag a[kCache];
+#pragma unroll
+            for (int i = 0; i < kCache; ++i)
+                a[i] = *reinterpret_cast<const Frag*>(at + i * kPlane + 512 * c + 16 * ((lane & 31) ^ c));
+            s = products(a, q[ks], s);
+        }
+        return s;
+    }
+    static __device__ __forceinline__ void accumulate(const floatx16& s, const unsigned char* at, int lane, floatx16 (&o)[2])
+    {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            floatx8 pv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pv[e] = s[8 * ks + e];
+            Frag f[P::kN];
+            P::split(pv, f);
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt) {
+                Frag a[kCache];
+#pragma unroll
+                for (int i = 0; i < kCache; ++i)
+                    a[i] = *reinterpret_cast<const Frag*>(at + (kCache + i) * kPlane + 2048 * dt + 1024 * ks + 16 * lane);
+                o[dt] = products(a, f, o[dt]);
+            }
+        }
+    }
+};
+
+// Rows of one sequence and kv head, 128 of them: (token, head) pairs in order,
+// 32 to a wave.  A work item is such a tile of rows over a range of key tiles;
+// its waves share the tiles in LDS, double-buffered, the next one's rows
+// on their way in registers while the waves compute.
+// kSmall: pages of fewer than 8 positions, whose rows are looked up by each
+// lane; else the eight rows that a wave loads lie in one page.
+template <int kType, bool kSmall, int kMaxSeq>
+__global__ __launch_bounds__(256) void paged_chunk_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
+{
+    typedef typename Elem<kType>::T T;
+    typedef ChunkTile<kType> Tile;
+    typedef Pieces<kType> P;
+    typedef typename P::Frag Frag;
+    constexpr int kKeys = Tile::kKeys, kSub = Tile::kSub;
+    __shared__ __align__(16) unsigned char s_kv[2][kSub][Tile::kBytes];
+    __shared__ unsigned s_there[2][kSub];  // bit i: key i of the plane is there
+    __shared__ int s_last;
+    const int item = blockIdx.x;
+    const int rank = rank_of(b, p.n_seq, item), seq = b.id(rank);
+    const int pos = b.pos[seq], n_tok = b.tok[seq + 1] - b.tok[seq], len = pos + n_tok;
+    const int n_rows = n_tok * p.gqa, n_rt = (n_rows + kChunkRows - 1) / kChunkRows;
+    // Row tiles last first (they see most keys); the items of one tile next to
+    // each other, so that with a multiple of 8 of them, or a divisor, the row
+    // tiles that read one range of keys of one head run on the same XCDs.
+    const int local = item - b.first[rank];
+    const int n_combo = (b.first[rank + 1] - b.first[rank]) / n_rt;
+    const int rt = n_rt - 1 - local / n_combo, combo = local % n_combo;
+    const int kvh = combo % p.n_head_kv, split = combo / p.n_head_kv;
+    const int row0 = rt * kChunkRows, last_row = min(row0 + kChunkRows, n_rows) - 1;
+    const int last_key = pos + last_row / p.gqa;
+    const int n_tiles = last_key / kKeys + 1;
+    const int n_split = (n_tiles + p.split_tiles - 1) / p.split_tiles;
+    if (split >= n_split) return;  // the whole workgroup
+    const int tile0 = split * p.split_tiles, tile_end = min(tile0 + p.split_tiles, n_tiles);
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kWave - 1);
+    const int col = lane & 31, half = lane >> 5;
+    const int* const table = p.pool.table + (long long)seq * p.pool.table_stride;
+    const int kv_dim = p.n_head_kv * kHeadDim, head_off = kvh * kHeadDim;
+    const int kk = threadIdx.x >> 3, kc = threadIdx.x & 7;   // this thread's piece of K
+    const int vg = threadIdx.x >> 5, vi = threadIdx.x & 31;  // and of V
+
+    typename Tile::KRaw k_raw[kSub];
+    typename Tile::VRaw v_raw[kSub][4];
+    unsigned there[kSub];  // the wave's eight rows
+    int page[kSub];
+    const auto look_up = [&](int tile) {
+        if constexpr (!kSmall) {
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) page[u] = table[min(tile * kKeys + 32 * u + 8 * wave, len - 1) >> p.pool.page_shift];
+        }
+    };
+    const auto load = [&](int tile) {
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            const int key = tile * kKeys + 32 * u + 8 * wave;  // the wave's first
+            if constexpr (kSmall) {
+                const auto at = [&](int j) { return j < len ? row_of(p.pool, table, j, kv_dim) : -1; };
+                const long long kr = at(tile * kKeys + 32 * u + kk);
+                const T* const ka = static_cast<const T*>(p.pool.k) + kr + head_off + 8 * kc;
+                k_raw[u] = kr >= 0 ? *reinterpret_cast<const typename Tile::KRaw*>(ka) : typename Tile::KRaw{};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const long long vr = at(tile * kKeys + 32 * u + 4 * vg + e);
+                    const T* const va = static_cast<const T*>(p.pool.v) + vr + head_off + 2 * vi;
+                    v_raw[u][e] = vr >= 0 ? *reinterpret_cast<const typename Tile::VRaw*>(va) : typename Tile::VRaw{};
+                }
+                const unsigned long long m = __ballot(kr >= 0);  // eight lanes to a key
+                there[u] = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) there[u] |= (unsigned)(m >> (8 * i) & 1) << i;
+            } else {
+                const bool seen = key < len && (unsigned)page[u] < (unsigned)p.pool.n_pages;
+                const long long at = seen ? (long long)page[u] * p.pool.page_stride +
+                                                (long long)(key & ((1 << p.pool.page_shift) - 1)) * kv_dim + head_off
+                                          : 0;
+                const unsigned row_bytes = kv_dim * sizeof(T);
+                const int rows = min(8, len - key);
+                const unsigned bytes = seen ? (rows - 1) * row_bytes + kHeadDim * (unsigned)sizeof(T) : 0;
+                const auto rk = rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(p.pool.k) + at), bytes});
+                const auto rv = rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(p.pool.v) + at), bytes});
+                const unsigned ko = (kk & 7) * row_bytes + 8 * kc * sizeof(T);
+                if constexpr (kType == kKvF32) {
+                    const floatx4 x = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko, 0, 0));
+                    const floatx4 y = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko + 16, 0, 0));
+                    k_raw[u] = floatx8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                } else {
+                    k_raw[u] = __builtin_amdgcn_raw_buffer_load_b128(rk, ko, 0, 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned vo = (4 * (vg & 1) + e) * row_bytes + 2 * vi * sizeof(T);
+                    if constexpr (kType == kKvF32)
+                        v_raw[u][e] = __builtin_bit_cast(floatx2, __builtin_amdgcn_raw_buffer_load_b64(rv, vo, 0, 0));
+                    else
+                        v_raw[u][e] = __builtin_amdgcn_raw_buffer_load_b32(rv, vo, 0, 0);
+                }
+                there[u] = seen ? 255 : 0;
+            }
+        }
+    };
+    const auto store = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            Tile::store(k_raw[u], v_raw[u], s_kv[buf][u], kk, kc, vi, vg);
+            if (lane == 0) reinterpret_cast<unsigned char*>(&s_there[buf][u])[wave] = (unsigned char)there[u];
+        }
+    };
+
+    look_up(tile0);
+    load(tile0);
+    look_up(min(tile0 + 1, n_tiles - 1));
+
+    // The row's query: lane (half, col) holds dimensions 16 s + 8 half .. + 7 for k step s.
+    const int row = min(row0 + 32 * wave + col, n_rows - 1), t = row / p.gqa, qpos = pos + t;
+    const long long q_at = ((long long)(b.tok[seq] + t) * p.n_head + kvh * p.gqa + row - t * p.gqa) * kHeadDim;
+    const bool real = row0 + 32 * wave + col < n_rows;
+    Frag q[4][P::kN];
+    float down = 1.f;
+    {
+        const float* const cs = reinterpret_cast<const float*>(p.rope + (long long)qpos * kPairs);
+        floatx4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = scaled_q4(p.q + q_at, cs, 16 * (i >> 1) + 8 * half + 4 * (i & 1), p.rotate, p.scale_log2);
+        float up = 1.f;
+        if constexpr (P::kScaled) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, __builtin_fabsf(x[i][e]));
+            row_scale(max_xor32(top), up, down);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            floatx8 v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = x[2 * s + (e >> 2)][e & 3] * up;
+            P::split(v, q[s]);
+        }
+    }
+    // Keys that some row of the wave sees, and those that all of them do.
+    const int wave_row = row0 + 32 * wave;
+    const int wave_last = wave_row < n_rows ? pos + min(wave_row + 31, n_rows - 1) / p.gqa : -1;
+    const int wave_first = pos + min(wave_row, n_rows - 1) / p.gqa;
+
+    store(0);
+    __syncthreads();
+    floatx16 o[2] = {};
+    float m_run = -INFINITY, l_run = 0.f;
+    constexpr float kShift = P::kShift;
+    for (int tile = tile0; tile < tile_end; ++tile) {
+        const int buf = (tile - tile0) & 1;
+        if (tile + 1 < tile_end) {
+            load(tile + 1);
+            look_up(min(tile + 2, n_tiles - 1));
+        }
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            const int key = tile * kKeys + 32 * u;
+            const unsigned seen = __builtin_amdgcn_readfirstlane(s_there[buf][u]);
+            if (key > wave_last || seen == 0) continue;  // uniform over the wave
+            floatx16 s = Tile::scores(s_kv[buf][u], q, lane);
+            if constexpr (P::kScaled) s *= down;
+            if (key + 31 > wave_first || seen != ~0u) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = 16 * (r >> 3) + 8 * half + (r & 7);
+                    s[r] = key + j <= qpos && (seen >> j & 1) ? s[r] : -INFINITY;
+                }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+            mx = max_xor32(mx);
+            if (__any(mx > m_run + kRescaleSlack)) {
+                const float m_new = fmaxf(m_run, mx);
+                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+                m_run = m_new;
+                l_run *= alpha;
+                o[0] *= alpha;
+                o[1] *= alpha;
+            }
+            const float m_use = m_run == -INFINITY ? 0.f : m_run - kShift;
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = __builtin_amdgcn_exp2f(s[r] - m_use);
+                sum += s[r];
+            }
+            l_run += sum;
+            Tile::accumulate(s, s_kv[buf][u], lane, o);
+        }
+        if (tile + 1 < tile_end) store(buf ^ 1);  // read before the barrier that ended the last step
+        __syncthreads();
+    }
+    l_run = sum_xor32(l_run);
+
+    if (n_split > 1) {
+        const auto part_of = [&](int s) {
+            const long long i = b.first[rank] + (long long)(n_rt - 1 - rt) * n_combo + s * p.n_head_kv + kvh;
+            return __builtin_amdgcn_make_buffer_rsrc(p.part + i * (kChunkStateBytes / 4) + wave * (64 * 34), 0, 64 * 34 * 4, kRawBufferWord3);
+        };
+        const auto mine = part_of(split);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            floatx4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = o[i >> 2][4 * (i & 3) + e];
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, x), mine, 1024 * i + 16 * lane, 0, kDeviceScope);
+        }
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uintx2, make_float2(m_run, l_run)), mine, 8192 + 8 * lane, 0, kDeviceScope);
+        if (!last_to_arrive(p.counters + b.first[rank] + (n_rt - 1 - rt) * n_combo + kvh, n_split, s_last)) return;
+        m_run = -INFINITY;
+        l_run = 0.f;
+        o[0] = o[1] = floatx16{};
+        for (int i = 0; i < n_split; ++i) {
+            const auto rs = part_of(i);
+            floatx4 x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[j] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rs, 1024 * j + 16 * lane, 0, kDeviceScope));
+            const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8192 + 8 * lane, 0, kDeviceScope));
+            const float m_new = fmaxf(m_run, ml.x);
+            const float fa = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+            const float fb = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m_new);
+            m_run = m_new;
+            l_run = l_run * fa + ml.y * fb;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[0][e] = o[0][e] * fa + x[e >> 2][e & 3] * fb;
+                o[1][e] = o[1][e] * fa + x[4 + (e >> 2)][e & 3] * fb;
+            }
+        }
+    }
+    const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+    bool bad = not_finite(l_run);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+        o[dt] *= inv;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) bad |= not_finite(o[dt][e]);
+    }
+    // The row as a whole: its query may lie where its output goes.
+    const unsigned long long bads = __ballot(real && bad);
+    const unsigned bad_rows = (unsigned)bads | (unsigned)(bads >> 32);
+    if (real && !(bad_rows >> col & 1)) {  // o[dt][4 a + e] = dimension 16 a + 8 half + 2 e + dt
+        float* const orow = p.out + q_at + 8 * half;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            stg4(orow + 16 * a, make_float4(o[0][4 * a], o[1][4 * a], o[0][4 * a + 1], o[1][4 * a + 1]));
+            stg4(orow + 16 * a + 4, make_float4(o[0][4 * a + 2], o[1][4 * a + 2], o[0][4 * a + 3], o[1][4 * a + 3]));
+        }
+    }
+    // Rows that met something infinite or NaN, seen or not, once more in plain fp32.
+    for (unsigned rows = bad_rows; rows; rows &= rows - 1) {
+        const int i = wave_row + __builtin_ctz(rows), ti = i / p.gqa;
+        const long long at = ((long long)(b.tok[seq] + ti) * p.n_head + kvh * p.gqa + i - ti * p.gqa) * kHeadDim;
+        const float x = q_lane(p.q + at, p.rope + (long long)(pos + ti) * kPairs, p.rotate, p.scale_log2);
+        p.out[at + lane] = plain_row<kType>(p.pool, table, kv_dim, head_off, pos + ti, x);
+    }
 }
 
 // f(batch) with the kernel argument block of the smallest size that holds n
@@ -237,13 +1060,92 @@ hipError_t launch_paged_append(const PagedAppendParams& p, const PagedBatch& b, 
     });
 }
 
-hipError_t launch_paged_attention(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s)
+// A range of keys is at least one tile per wave; beyond that, ranges such that
+// the launch has about four workgroups per CU.
+void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, PagedPlan* p)
+{
+    PagedBatch& b = p->batch;
+    const auto tiles_of = [&](int s) {
+        const int n_tok = b.tok[s + 1] - b.tok[s];
+        return n_tok > 0 && n_tok * gqa <= kStreamRows ? (b.pos[s] + n_tok + kStreamTile - 1) / kStreamTile : 0;
+    };
+    long long total = 0;
+    for (int s = 0; s < n_seq; ++s) total += tiles_of(s);
+    const long long target = 4ll * n_cu;
+    const long long split = std::max<long long>(4, (total * n_head_kv + target - 1) / target);
+    p->split_tiles = static_cast<int>((split + 3) / 4 * 4);
+    p->shared = false;
+    long long at = 0;
+    for (int s = 0; s < n_seq; ++s) {
+        b.first[s] = static_cast<int>(at);
+        b.set_id(s, s);
+        const int n = (tiles_of(s) + p->split_tiles - 1) / p->split_tiles;
+        p->shared |= n > 1;
+        at += static_cast<long long>(n) * n_head_kv;
+    }
+    b.first[n_seq] = p->n_items = static_cast<int>(at);
+}
+
+int chunk_tile(int type)
+{
+    return type == kKvF32 ? ChunkTile<kKvF32>::kKeys : ChunkTile<kKvF16>::kKeys;
+}
+
+// Row tiles over all their keys where they are enough for three workgroups
+// per CU, else over ranges of at least eight tiles.
+void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* p)
+{
+    PagedBatch& b = p->batch;
+    const int keys = chunk_tile(type);
+    const auto rows_of = [&](int s) {
+        const long long rows = static_cast<long long>(b.tok[s + 1] - b.tok[s]) * gqa;
+        return rows > kStreamRows ? rows : 0;
+    };
+    long long total = 0;
+    for (int s = 0; s < n_seq; ++s) {
+        const long long rows = rows_of(s);
+        for (long long r = 0; r < rows; r += kChunkRows)
+            total += (b.pos[s] + (std::min(r + kChunkRows, rows) - 1) / gqa) / keys + 1;
+    }
+    const long long target = 3ll * n_cu;
+    p->split_tiles = static_cast<int>(std::max<long long>(8, (total * n_head_kv + target - 1) / target));
+    p->shared = false;
+    long long at = 0;
+    for (int s = 0; s < n_seq; ++s) {
+        b.first[s] = static_cast<int>(at);
+        b.set_id(s, s);
+        const long long rows = rows_of(s);
+        if (!rows) continue;
+        const int last = b.pos[s] + b.tok[s + 1] - b.tok[s] - 1;
+        const long long splits = (last / keys + p->split_tiles) / p->split_tiles;
+        p->shared |= splits > 1;
+        at += (rows + kChunkRows - 1) / kChunkRows * splits * n_head_kv;
+    }
+    b.first[n_seq] = p->n_items = static_cast<int>(at);
+}
+
+hipError_t launch_paged_stream(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s)
 {
     return with_type(p.pool.type, [&](auto type) {
         return with_batch(b, p.n_seq, [&](const auto& seqs) {
             constexpr int kMax = sizeof(seqs.pos) / sizeof(int);
-            hipLaunchKernelGGL((paged_attention_kernel<type.value, kMax>), dim3((p.n_items + 3) / 4), dim3(256), 0, s,
-                               p, seqs);
+            if (p.pool.page_shift < 4)
+                hipLaunchKernelGGL((paged_stream_kernel<type.value, true, kMax>), dim3(p.n_items), dim3(256), 0, s, p, seqs);
+            else
+                hipLaunchKernelGGL((paged_stream_kernel<type.value, false, kMax>), dim3(p.n_items), dim3(256), 0, s, p, seqs);
+        });
+    });
+}
+
+hipError_t launch_paged_chunk(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s)
+{
+    return with_type(p.pool.type, [&](auto type) {
+        return with_batch(b, p.n_seq, [&](const auto& seqs) {
+            constexpr int kMax = sizeof(seqs.pos) / sizeof(int);
+            if (p.pool.page_shift < 3)
+                hipLaunchKernelGGL((paged_chunk_kernel<type.value, true, kMax>), dim3(p.n_items), dim3(256), 0, s, p, seqs);
+            else
+                hipLaunchKernelGGL((paged_chunk_kernel<type.value, false, kMax>), dim3(p.n_items), dim3(256), 0, s, p, seqs);
         });
     });
 }
