@@ -137,10 +137,8 @@ struct tla_engine {
     size_t kvp_bytes = 0;
     float* pf_part = nullptr;     // its states of workgroups that share a query tile
     int* pf_counters = nullptr;   // and their arrivals, zero between launches
-    unsigned long long* best = nullptr;  // logits: the best of each slice of each row
-    size_t best_bytes = 0;
-    int* best_counters = nullptr;        // and their arrivals, zero between launches
-    size_t n_best_counters = 0;
+    int* best = nullptr;     // logits: the best of each slice of each row and their
+    size_t n_best = 0;       // arrivals, zero between launches (words)
     int* argmax_slot = nullptr;
     unsigned long long* amax_keys = nullptr;  // kAmaxSlots keys (tla_matmul_argmax)
     long long opt_split = 0;
@@ -470,7 +468,6 @@ int tla_engine_destroy(tla_engine* e)
     if (e->kvp) (void)hipFree(e->kvp);
     if (e->pf_part) (void)hipFree(e->pf_part);
     if (e->best) (void)hipFree(e->best);
-    if (e->best_counters) (void)hipFree(e->best_counters);
     if (e->argmax_slot) (void)hipFree(e->argmax_slot);
     if (e->amax_keys) (void)hipFree(e->amax_keys);
     if (e->rope) (void)hipFree(e->rope);
@@ -1464,16 +1461,16 @@ int tla_logits_process(tla_engine* e, int n_seq, int n_vocab, const tla_logit_ru
     p.out = out_dev;
     p.tokens = tokens_dev;
     p.n_vocab = n_vocab;
-    p.n_slices = logits_slices(n_vocab);
+    p.slice = logits_slice(n_seq, n_vocab, e->n_cu);
+    p.n_slices = (n_vocab + p.slice - 1) / p.slice;
     if (static_cast<long long>(n_seq) * p.n_slices > 0x7fffffff)
         return fail(TLA_ERR_UNSUPPORTED, "%d rows of %d logits", n_seq, n_vocab);
-    if (tokens_dev) {
-        if (int rc = ensure_buf(e, reinterpret_cast<void**>(&e->best), e->best_bytes,
-                                sizeof(unsigned long long) * n_seq * p.n_slices, "logits' best tokens"))
-            return rc;
-        if (int rc = ensure_counters(e, &e->best_counters, e->n_best_counters, n_seq)) return rc;
-        p.best = e->best;
-        p.counters = e->best_counters;
+    if (tokens_dev && p.n_slices > 1) {
+        // rows' slots (two words each), then their counters: zero between launches
+        const size_t slots = static_cast<size_t>(n_seq) * p.n_slices;
+        if (int rc = ensure_counters(e, &e->best, e->n_best, 2 * slots + n_seq)) return rc;
+        p.best = reinterpret_cast<unsigned long long*>(e->best);
+        p.counters = e->best + 2 * slots;
     }
     return launch(e, TLA_KERNEL_LOGITS, "logits", [&] { return launch_logits_process(p, n_seq, e->stream); });
 }

@@ -10,16 +10,17 @@ struct LogitsParams {
     float* out;      // may be x
     int* tokens;     // [n_seq], or NULL
     int n_vocab;
+    int slice;       // logits per workgroup (logits_slice)
     int n_slices;    // workgroups per row
     tla_logit_rules rules;
-    // With tokens: each workgroup's best (an argmax key), [n_seq][n_slices],
-    // and the rows' arrivals, zero between launches.
+    // With tokens and several slices: each workgroup's best (an argmax key),
+    // [n_seq][n_slices], and the rows' arrivals; zero between launches.
     unsigned long long* best;
     int* counters;
 };
 
-// Workgroups per row of n_vocab logits.
-int logits_slices(int n_vocab);
+// Logits per workgroup.
+int logits_slice(int n_seq, int n_vocab, int n_cu);
 hipError_t launch_logits_process(const LogitsParams& p, int n_seq, hipStream_t s);
 hipError_t load_logits_code();
 
