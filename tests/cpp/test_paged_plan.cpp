@@ -1,0 +1,82 @@
+// Plans of paged attention on the CPU: every query row of every sequence is
+// served by exactly one kernel, every key tile by exactly one work item of its
+// rows, as the kernels take the items apart.
+#include <cstdio>
+#include <cstdlib>
+#include <memory>
+#include <random>
+#include <vector>
+
+#include "paged_plan.h"
+
+using namespace tla;
+
+#define CHECK(x)                                                          \
+    do {                                                                  \
+        if (!(x)) {                                                       \
+            std::printf("line %d: %s fails (case %d)\n", __LINE__, #x, n_case); \
+            std::exit(1);                                                 \
+        }                                                                 \
+    } while (0)
+
+int main()
+{
+    std::mt19937 rng(1);
+    const auto pick = [&](int lo, int hi) { return lo + static_cast<int>(rng() % static_cast<unsigned>(hi - lo + 1)); };
+    for (int n_case = 0; n_case < 3000; ++n_case) {
+        const int n_seq = n_case % 5 == 0 ? 1 : pick(1, n_case % 7 == 0 ? 256 : 12);
+        const int gqa = pick(1, 16), hkv = pick(1, 8), n_cu = n_case % 11 == 0 ? 8 : 256;
+        const int type = n_case % 3 == 0 ? kKvF32 : n_case % 3 == 1 ? kKvF16 : kKvBF16;
+        auto plan = std::make_unique<PagedPlan>();
+        PagedBatch& b = plan->batch;
+        int t = 0;
+        for (int s = 0; s < n_seq; ++s) {
+            b.pos[s] = pick(0, 3) ? pick(0, 1 << pick(0, 14)) : 0;
+            b.tok[s] = t;
+            t += pick(0, 3) == 0 ? 0 : pick(0, 2) ? 1 : pick(1, 1 << pick(0, 11));
+        }
+        b.tok[n_seq] = t;
+        std::vector<int> served(n_seq, 0);
+        for (const bool chunk : {true, false}) {
+            if (chunk)
+                plan_chunk(n_seq, hkv, gqa, n_cu, type, plan.get());
+            else
+                plan_stream(n_seq, hkv, gqa, n_cu, plan.get());
+            if (plan->n_items == 0) continue;
+            CHECK(plan->n_items == b.first[n_seq] && b.first[0] == 0);
+            bool shared = false;
+            for (int r = 0; r < n_seq; ++r) {
+                const int s = b.id(r), items = b.first[r + 1] - b.first[r];
+                CHECK(items >= 0);
+                const int n_tok = b.tok[s + 1] - b.tok[s], len = b.pos[s] + n_tok, rows = n_tok * gqa;
+                if (!items) continue;
+                ++served[s];
+                CHECK(items % hkv == 0);
+                if (!chunk) {
+                    CHECK(rows >= 1 && rows <= kStreamRows);
+                    const int n_split = items / hkv, n_tiles = (len + kStreamTile - 1) / kStreamTile;
+                    const int per = (n_tiles + n_split - 1) / n_split;
+                    CHECK(static_cast<long long>(per) * n_split >= n_tiles);
+                    shared |= n_split > 1;
+                    CHECK(n_split == 1 || per >= 2);
+                } else {
+                    CHECK(rows > kStreamRows);
+                    const int n_rt = (rows + kChunkRows - 1) / kChunkRows;
+                    CHECK(items % (n_rt * hkv) == 0);
+                    const int splits = items / (n_rt * hkv), keys = chunk_tile(type);
+                    for (int rt = 0; rt < n_rt; rt += 1 + n_rt / 7) {
+                        const int last_row = std::min((rt + 1) * kChunkRows, rows) - 1;
+                        const int n_tiles = (b.pos[s] + last_row / gqa) / keys + 1;
+                        const int n_split = (n_tiles + plan->split_tiles - 1) / plan->split_tiles;
+                        CHECK(n_split >= 1 && n_split <= splits);
+                        shared |= n_split > 1;
+                    }
+                }
+            }
+            CHECK(plan->shared || !shared);
+        }
+        for (int s = 0; s < n_seq; ++s) CHECK(served[s] == (b.tok[s + 1] > b.tok[s] ? 1 : 0));
+    }
+    std::printf("plans hold\n");
+    return 0;
+}

@@ -17,6 +17,7 @@
 #include "batch.h"
 #include "logits.h"
 #include "paged.h"
+#include "paged_plan.h"
 #include "prefill.h"
 #include "tla_internal.h"
 

@@ -90,9 +90,8 @@ struct PagedPlan {
 // Bytes of one work item's softmax state.
 constexpr int kStreamStateBytes = 64 * 18 * 4;
 constexpr int kChunkStateBytes = 4 * 64 * 34 * 4;
-int chunk_tile(int type);  // keys per tile of paged_chunk_kernel
-void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, PagedPlan* p);
-void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* p);
+// Keys per tile of paged_chunk_kernel.
+constexpr int chunk_tile(int type) { return type == kKvF32 ? 32 : 64; }
 hipError_t launch_paged_stream(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s);
 hipError_t launch_paged_chunk(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s);
 

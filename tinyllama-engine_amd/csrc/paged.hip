@@ -1,7 +1,5 @@
 // Paged KV cache for gfx950: append of new keys (rotated) and values, and
 // attention of new tokens over their sequences' pages.
-#include <algorithm>
-
 #include "bf16_split.h"
 #include "lane_math.h"
 #include "paged.h"
@@ -205,7 +203,10 @@ struct Pieces<kKvF16> {
     static __device__ __forceinline__ void split(floatx8 v, Frag (&o)[kN])
     {
         o[0] = __builtin_convertvector(v, f16x8);
-        o[1] = __builtin_convertvector(v - __builtin_convertvector(o[0], floatx8), f16x8);
+        floatx8 r;  // exact; one v_fma_mix each
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = fmaf((float)o[0][e], -1.f, v[e]);
+        o[1] = __builtin_convertvector(r, f16x8);
     }
     static __device__ __forceinline__ floatx4 mfma16(Frag a, Frag b, floatx4 c)
     {
@@ -307,26 +308,27 @@ template <int kType>
 struct StreamTile {
     typedef Pieces<kType> P;
     typedef typename P::Frag Frag;
-    // k step ks: dimensions 16 g + 8 ks .. + 7
+    // k step ks: dimensions 32 ks + 8 g .. + 7, so that one load instruction
+    // takes 64 consecutive bytes of each row
     uintx4 k[2][2];
     uintx2 v[8];
     struct Query {
         Frag f[2][P::kN];
         float down;
     };
-    static constexpr int kKeyBytes = 16;
-    template <class L>
+    // x[i] of Query::query: dimensions q_dim(i, g) .. + 3
+    static __device__ __forceinline__ int q_dim(int i, int g) { return 32 * (i >> 1) + 8 * g + 4 * (i & 1); }
+    template <class L>  // load16(o): 16 bytes at byte o + 16 g of row c
     __device__ __forceinline__ void load_k(int hf, L&& load16)
     {
         k[hf][0] = load16(0);
-        k[hf][1] = load16(16);
+        k[hf][1] = load16(64);
     }
     template <class L>
     __device__ __forceinline__ void load_v(int hf, int r, L&& load8)
     {
         v[4 * hf + r] = load8();
     }
-    // x: dimensions 16 g .. + 15 of the row
     static __device__ __forceinline__ void query(const floatx4 (&x)[4], Query& q)
     {
         float up = 1.f;
@@ -373,7 +375,7 @@ struct StreamTile {
     }
 };
 // fp32 elements: the fp32 MFMA, exact products at the rate that one pass over
-// the keys needs.  Its 16 k steps take dimensions 16 g + i.
+// the keys needs.  Its k step 4 i + e takes dimension 16 i + 4 g + e.
 template <>
 struct StreamTile<kKvF32> {
     floatx4 k[2][4];
@@ -382,12 +384,12 @@ struct StreamTile<kKvF32> {
         floatx4 x[4];
         float down;
     };
-    static constexpr int kKeyBytes = 32;
+    static __device__ __forceinline__ int q_dim(int i, int g) { return 16 * i + 4 * g; }
     template <class L>
     __device__ __forceinline__ void load_k(int hf, L&& load16)
     {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[hf][i] = __builtin_bit_cast(floatx4, load16(16 * i));
+        for (int i = 0; i < 4; ++i) k[hf][i] = __builtin_bit_cast(floatx4, load16(64 * i));
     }
     template <class L>
     __device__ __forceinline__ void load_v(int hf, int r, L&& load16)
@@ -420,15 +422,17 @@ struct StreamTile<kKvF32> {
 };
 
 // Rows of one sequence and kv head: up to 16 (token, head) pairs, row c being
-// token c / gqa, head c % gqa of the kv head.  One work item is a range of
-// split_tiles 32-key tiles, its four waves taking every fourth tile each, with
+// token c / gqa, head c % gqa of the kv head.  One work item is an equal part of
+// the unit's 32-key tiles, its four waves taking every fourth tile each, with
 // no word to each other until the end: then the waves' states meet in LDS,
 // and the items of one unit in the workspace, where the last to arrive adds
-// them in order.
+// them in order.  A wave holds one tile: its keys' registers take the next
+// tile's as soon as the scores are formed, its values' after P.V.  The other
+// waves of the SIMD cover the wait.
 // kSmall: pages of fewer than 16 positions, whose rows are looked up one by
 // one; else each half of a tile lies in one page, looked up by the wave.
 template <int kType, bool kSmall, int kMaxSeq>
-__global__ __launch_bounds__(256) void paged_stream_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void paged_stream_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
 {
     typedef typename Elem<kType>::T T;
     typedef StreamTile<kType> Tile;
@@ -455,99 +459,114 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const PagedAttentionP
     const float* const cs = reinterpret_cast<const float*>(p.rope + (long long)qpos * kPairs);
     if (threadIdx.x < 16) s_bad[threadIdx.x] = 0;
 
-    Tile cur, next;
-    bool cur_seen[2], next_seen[2];        // kSmall: none; the halves' pages are there
-    unsigned cur_mask = 0, next_mask = 0;  // kSmall: bit 4 hf + r, the row is there
-    const auto look_up = [&](int tile, int (&page)[2]) {
+    // The tile's operands, and which of its keys are there: kSmall: bit 4 hf + r
+    // of mask, the lane's key 4 g + r of half hf; else the halves' pages.
+    Tile kv;
+    struct There {
+        unsigned mask;
+        bool half[2];
+    } there = {}, next = {};
+    int page[2] = {};
+    const auto look_up = [&](int tile) {
         if constexpr (!kSmall) {
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) page[hf] = table[min(tile * kStreamTile + 16 * hf, len - 1) >> p.pool.page_shift];
         }
     };
-    const auto load = [&](int tile, const int (&page)[2], Tile& d, bool (&seen)[2], unsigned& mask) {
-        if constexpr (kSmall) {
-            mask = 0;
+    const unsigned row_bytes = kv_dim * sizeof(T);
+    const auto rows_of = [&](const void* pool, int tile, int hf) {  // of the page looked up last
+        const int key = tile * kStreamTile + 16 * hf;
+        const bool seen = key < len && (unsigned)page[hf] < (unsigned)p.pool.n_pages;
+        next.half[hf] = seen;
+        const long long at = (long long)page[hf] * p.pool.page_stride +
+                             (long long)(key & ((1 << p.pool.page_shift) - 1)) * kv_dim + head_off;
+        return rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(pool) + (seen ? at : 0)),
+                        seen ? (min(16, len - key) - 1) * row_bytes + kHeadDim * (unsigned)sizeof(T) : 0});
+    };
+    const auto load_k = [&](int tile) {
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int kk = tile * kStreamTile + 16 * hf + c;
-                const long long kr = kk < len ? row_of(p.pool, table, kk, kv_dim) : -1;
-                const char* const ka = reinterpret_cast<const char*>(static_cast<const T*>(p.pool.k) + kr + head_off) + Tile::kKeyBytes * 2 * g;
-                d.load_k(hf, [&](int o) { return kr >= 0 ? *reinterpret_cast<const uintx4*>(ka + o) : uintx4{}; });
+        for (int hf = 0; hf < 2; ++hf) {
+            if constexpr (kSmall) {
+                const int key = tile * kStreamTile + 16 * hf + c;
+                const long long at = key < len ? row_of(p.pool, table, key, kv_dim) : -1;
+                const char* const from =
+                    reinterpret_cast<const char*>(static_cast<const T*>(p.pool.k) + at + head_off) + 16 * g;
+                kv.load_k(hf, [&](int o) { return at >= 0 ? *reinterpret_cast<const uintx4*>(from + o) : uintx4{}; });
+            } else {
+                const auto rs = rows_of(p.pool.k, tile, hf);
+                kv.load_k(hf, [&](int o) {
+                    return __builtin_amdgcn_raw_buffer_load_b128(rs, c * row_bytes + 16 * g + o, 0, 0);
+                });
+            }
+        }
+    };
+    const auto load_v = [&](int tile) {
+        typedef std::conditional_t<kType == kKvF32, uintx4, uintx2> V;
+        next.mask = 0;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            if constexpr (kSmall) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int vk = tile * kStreamTile + 16 * hf + 4 * g + r;
-                    const long long vr = vk < len ? row_of(p.pool, table, vk, kv_dim) : -1;
-                    const T* const va = static_cast<const T*>(p.pool.v) + vr + head_off + 4 * c;
-                    typedef std::conditional_t<kType == kKvF32, uintx4, uintx2> V;
-                    d.load_v(hf, r, [&] { return vr >= 0 ? *reinterpret_cast<const V*>(va) : V{}; });
-                    mask |= vr >= 0 ? 1u << (4 * hf + r) : 0u;
+                    const int key = tile * kStreamTile + 16 * hf + 4 * g + r;
+                    const long long at = key < len ? row_of(p.pool, table, key, kv_dim) : -1;
+                    const T* const from = static_cast<const T*>(p.pool.v) + at + head_off + 4 * c;
+                    kv.load_v(hf, r, [&] { return at >= 0 ? *reinterpret_cast<const V*>(from) : V{}; });
+                    next.mask |= at >= 0 ? 1u << (4 * hf + r) : 0u;
                 }
-            }
-        } else {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int key = tile * kStreamTile + 16 * hf;
-                seen[hf] = key < len && (unsigned)page[hf] < (unsigned)p.pool.n_pages;
-                const long long at = (long long)page[hf] * p.pool.page_stride +
-                                     (long long)(key & ((1 << p.pool.page_shift) - 1)) * kv_dim + head_off;
-                const unsigned row_bytes = kv_dim * sizeof(T);
-                const unsigned bytes = seen[hf] ? (min(16, len - key) - 1) * row_bytes + kHeadDim * (unsigned)sizeof(T) : 0;
-                const auto rk = rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(p.pool.k) + (seen[hf] ? at : 0)), bytes});
-                const auto rv = rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(p.pool.v) + (seen[hf] ? at : 0)), bytes});
-                d.load_k(hf, [&](int o) {
-                    return __builtin_amdgcn_raw_buffer_load_b128(rk, c * row_bytes + Tile::kKeyBytes * 2 * g + o, 0, 0);
-                });
+            } else {
+                const auto rs = rows_of(p.pool.v, tile, hf);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    d.load_v(hf, r, [&] {
+                    kv.load_v(hf, r, [&] {
                         if constexpr (kType == kKvF32)
-                            return __builtin_amdgcn_raw_buffer_load_b128(rv, (4 * g + r) * row_bytes + 16 * c, 0, 0);
+                            return __builtin_amdgcn_raw_buffer_load_b128(rs, (4 * g + r) * row_bytes + 16 * c, 0, 0);
                         else
-                            return __builtin_amdgcn_raw_buffer_load_b64(rv, (4 * g + r) * row_bytes + 8 * c, 0, 0);
+                            return __builtin_amdgcn_raw_buffer_load_b64(rs, (4 * g + r) * row_bytes + 8 * c, 0, 0);
                     });
             }
         }
     };
 
-    int tile = split * p.split_tiles + wave;
-    const int tile_end = min((split + 1) * p.split_tiles, n_tiles);
-    int page[2] = {};
+    const int per = (n_tiles + n_split - 1) / n_split;  // the unit's tiles in equal parts
+    int tile = split * per + wave;
+    const int tile_end = min((split + 1) * per, n_tiles);
     if (tile < tile_end) {  // first the keys, on whose way the query is rotated
-        look_up(tile, page);
-        load(tile, page, cur, cur_seen, cur_mask);
-        look_up(min(tile + 4, n_tiles - 1), page);
+        look_up(tile);
+        load_k(tile);
+        load_v(tile);
+        look_up(min(tile + 4, n_tiles - 1));
     }
     typename Tile::Query q;
     {
         floatx4 x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = scaled_q4(p.q + q_at, cs, 16 * g + 4 * i, p.rotate, p.scale_log2);
+        for (int i = 0; i < 4; ++i) x[i] = scaled_q4(p.q + q_at, cs, Tile::q_dim(i, g), p.rotate, p.scale_log2);
         Tile::query(x, q);
     }
     floatx4 o[4] = {};
     float m_run = -INFINITY, l_run = 0.f;
     constexpr float kShift = Pieces<kType>::kShift;
     for (; tile < tile_end; tile += 4) {
-        if (tile + 4 < tile_end) {
-            load(tile + 4, page, next, next_seen, next_mask);
-            look_up(min(tile + 8, n_tiles - 1), page);
-        }
+        const bool more = tile + 4 < tile_end;
+        there = next;
         floatx4 s[2];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) s[hf] = cur.scores(hf, q) * q.down;
+        for (int hf = 0; hf < 2; ++hf) s[hf] = kv.scores(hf, q);
+        if (more) load_k(tile + 4);  // into the registers just read
         const int key = tile * kStreamTile + 4 * g;
-        if (kSmall || (tile + 1) * kStreamTile > pos + 1 || !cur_seen[0] || !cur_seen[1]) {
+        if (kSmall || (tile + 1) * kStreamTile > pos + 1 || !there.half[0] || !there.half[1]) {
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const bool there = kSmall ? (cur_mask >> (4 * hf + r) & 1) != 0 : cur_seen[hf];
-                    s[hf][r] = there && key + 16 * hf + r <= qpos ? s[hf][r] : -INFINITY;
+                    const bool seen = kSmall ? (there.mask >> (4 * hf + r) & 1) != 0 : there.half[hf];
+                    s[hf][r] = seen && key + 16 * hf + r <= qpos ? s[hf][r] : -INFINITY;
                 }
         }
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        mx = max_xor32(max_xor16(mx));
+        mx = max_xor32(max_xor16(mx)) * q.down;
         // The running max moves only when a row's exceeds it by more than the
         // slack: most tiles do not rescale O.  A row that has seen nothing
         // keeps -inf; its probabilities are 0.
@@ -564,15 +583,13 @@ __global__ __launch_bounds__(256) void paged_stream_kernel(const PagedAttentionP
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[hf][r] = __builtin_amdgcn_exp2f(s[hf][r] - m_use);
+                s[hf][r] = __builtin_amdgcn_exp2f(fmaf(s[hf][r], q.down, -m_use));
                 l_run += s[hf][r];
             }
-        cur.accumulate(s, o);
-        if (tile + 4 < tile_end) {
-            cur = next;
-            cur_seen[0] = next_seen[0];
-            cur_seen[1] = next_seen[1];
-            cur_mask = next_mask;
+        kv.accumulate(s, o);
+        if (more) {
+            load_v(tile + 4);
+            look_up(min(tile + 8, n_tiles - 1));
         }
     }
     l_run = sum_xor32(sum_xor16(l_run));  // the lane groups summed different keys
@@ -656,8 +673,8 @@ struct ChunkTile {
     typedef Pieces<kType> P;
     typedef typename P::Frag Frag;
     static constexpr int kCache = kType == kKvF32 ? 3 : 1;  // planes of a cache element
-    static constexpr int kSub = kType == kKvF32 ? 1 : 2;    // 32-key planes per tile
-    static constexpr int kKeys = 32 * kSub;
+    static constexpr int kKeys = chunk_tile(kType);
+    static constexpr int kSub = kKeys / 32;                 // 32-key planes per tile
     static constexpr int kBytes = 2 * kCache * kPlane;      // K and V planes of 32 keys
     typedef std::conditional_t<kType == kKvF32, floatx8, uintx4> KRaw;                          // 8 dimensions of a key
     typedef std::conditional_t<kType == kKvF32, floatx2, unsigned> VRaw;                        // 2 dimensions of a key
@@ -749,7 +766,7 @@ struct ChunkTile {
 // kSmall: pages of fewer than 8 positions, whose rows are looked up by each
 // lane; else the eight rows that a wave loads lie in one page.
 template <int kType, bool kSmall, int kMaxSeq>
-__global__ __launch_bounds__(256) void paged_chunk_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void paged_chunk_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
 {
     typedef typename Elem<kType>::T T;
     typedef ChunkTile<kType> Tile;
@@ -905,7 +922,6 @@ __global__ __launch_bounds__(256) void paged_chunk_kernel(const PagedAttentionPa
             const unsigned seen = __builtin_amdgcn_readfirstlane(s_there[buf][u]);
             if (key > wave_last || seen == 0) continue;  // uniform over the wave
             floatx16 s = Tile::scores(s_kv[buf][u], q, lane);
-            if constexpr (P::kScaled) s *= down;
             if (key + 31 > wave_first || seen != ~0u) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -916,7 +932,7 @@ __global__ __launch_bounds__(256) void paged_chunk_kernel(const PagedAttentionPa
             float mx = s[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-            mx = max_xor32(mx);
+            mx = max_xor32(mx) * down;
             if (__any(mx > m_run + kRescaleSlack)) {
                 const float m_new = fmaxf(m_run, mx);
                 const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -929,7 +945,7 @@ __global__ __launch_bounds__(256) void paged_chunk_kernel(const PagedAttentionPa
             float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_amdgcn_exp2f(s[r] - m_use);
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], down, -m_use));
                 sum += s[r];
             }
             l_run += sum;
@@ -1058,70 +1074,6 @@ hipError_t launch_paged_append(const PagedAppendParams& p, const PagedBatch& b, 
                                seqs);
         });
     });
-}
-
-// A range of keys is at least one tile per wave; beyond that, ranges such that
-// the launch has about four workgroups per CU.
-void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, PagedPlan* p)
-{
-    PagedBatch& b = p->batch;
-    const auto tiles_of = [&](int s) {
-        const int n_tok = b.tok[s + 1] - b.tok[s];
-        return n_tok > 0 && n_tok * gqa <= kStreamRows ? (b.pos[s] + n_tok + kStreamTile - 1) / kStreamTile : 0;
-    };
-    long long total = 0;
-    for (int s = 0; s < n_seq; ++s) total += tiles_of(s);
-    const long long target = 4ll * n_cu;
-    const long long split = std::max<long long>(4, (total * n_head_kv + target - 1) / target);
-    p->split_tiles = static_cast<int>((split + 3) / 4 * 4);
-    p->shared = false;
-    long long at = 0;
-    for (int s = 0; s < n_seq; ++s) {
-        b.first[s] = static_cast<int>(at);
-        b.set_id(s, s);
-        const int n = (tiles_of(s) + p->split_tiles - 1) / p->split_tiles;
-        p->shared |= n > 1;
-        at += static_cast<long long>(n) * n_head_kv;
-    }
-    b.first[n_seq] = p->n_items = static_cast<int>(at);
-}
-
-int chunk_tile(int type)
-{
-    return type == kKvF32 ? ChunkTile<kKvF32>::kKeys : ChunkTile<kKvF16>::kKeys;
-}
-
-// Row tiles over all their keys where they are enough for three workgroups
-// per CU, else over ranges of at least eight tiles.
-void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* p)
-{
-    PagedBatch& b = p->batch;
-    const int keys = chunk_tile(type);
-    const auto rows_of = [&](int s) {
-        const long long rows = static_cast<long long>(b.tok[s + 1] - b.tok[s]) * gqa;
-        return rows > kStreamRows ? rows : 0;
-    };
-    long long total = 0;
-    for (int s = 0; s < n_seq; ++s) {
-        const long long rows = rows_of(s);
-        for (long long r = 0; r < rows; r += kChunkRows)
-            total += (b.pos[s] + (std::min(r + kChunkRows, rows) - 1) / gqa) / keys + 1;
-    }
-    const long long target = 3ll * n_cu;
-    p->split_tiles = static_cast<int>(std::max<long long>(8, (total * n_head_kv + target - 1) / target));
-    p->shared = false;
-    long long at = 0;
-    for (int s = 0; s < n_seq; ++s) {
-        b.first[s] = static_cast<int>(at);
-        b.set_id(s, s);
-        const long long rows = rows_of(s);
-        if (!rows) continue;
-        const int last = b.pos[s] + b.tok[s + 1] - b.tok[s] - 1;
-        const long long splits = (last / keys + p->split_tiles) / p->split_tiles;
-        p->shared |= splits > 1;
-        at += (rows + kChunkRows - 1) / kChunkRows * splits * n_head_kv;
-    }
-    b.first[n_seq] = p->n_items = static_cast<int>(at);
 }
 
 hipError_t launch_paged_stream(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s)
