@@ -59,6 +59,7 @@ int main()
                     CHECK(static_cast<long long>(per) * n_split >= n_tiles);
                     shared |= n_split > 1;
                     CHECK(n_split == 1 || per >= 2);
+                    CHECK(n_split <= kMaxStreamParts);
                 } else {
                     CHECK(rows > kStreamRows);
                     const int n_rt = (rows + kChunkRows - 1) / kChunkRows;

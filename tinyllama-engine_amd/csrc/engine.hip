@@ -1424,7 +1424,7 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
         if (plan.shared) {
             const size_t items = static_cast<size_t>(plan.n_items);
             if (int rc = ensure_ws(e, items * (chunk ? kChunkStateBytes : kStreamStateBytes))) return rc;
-            if (int rc = ensure_counters(e, &e->counters, e->n_counters, items)) return rc;
+            if (int rc = ensure_counters(e, &e->counters, e->n_counters, items * kCounterStride)) return rc;
             p.part = static_cast<float*>(e->ws);
             p.counters = e->counters;
         }
@@ -1469,7 +1469,7 @@ int tla_logits_process(tla_engine* e, int n_seq, int n_vocab, const tla_logit_ru
     if (tokens_dev && p.n_slices > 1) {
         // rows' slots (two words each), then their counters: zero between launches
         const size_t slots = static_cast<size_t>(n_seq) * p.n_slices;
-        if (int rc = ensure_counters(e, &e->best, e->n_best, 2 * slots + n_seq)) return rc;
+        if (int rc = ensure_counters(e, &e->best, e->n_best, 2 * slots + static_cast<size_t>(n_seq) * kRowCounterStride)) return rc;
         p.best = reinterpret_cast<unsigned long long*>(e->best);
         p.counters = e->best + 2 * slots;
     }

@@ -5,6 +5,10 @@
 
 namespace tla {
 
+// Words from one row's arrival counter to the next: device-scope atomics on one
+// line of memory wait for each other (0.11 us each).
+constexpr int kRowCounterStride = 64;
+
 struct LogitsParams {
     const float* x;  // [n_seq][n_vocab]
     float* out;      // may be x
@@ -14,7 +18,7 @@ struct LogitsParams {
     int n_slices;    // workgroups per row
     tla_logit_rules rules;
     // With tokens and several slices: each workgroup's best (an argmax key),
-    // [n_seq][n_slices], and the rows' arrivals; zero between launches.
+    // [n_seq][n_slices], and the rows' arrivals, kRowCounterStride apart; zero between launches.
     unsigned long long* best;
     int* counters;
 };

@@ -215,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsParams p)
             __hip_atomic_store(&p.best[(long long)row * p.n_slices + slice], best ? best : 1ull, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            last = __hip_atomic_fetch_add(&p.counters[row], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.n_slices - 1;
+            last = __hip_atomic_fetch_add(&p.counters[(long long)row * kRowCounterStride], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.n_slices - 1;
         }
         store();
         if (!__builtin_amdgcn_readfirstlane(last)) return;
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsParams p)
             best = max(best, k);
         }
         best = wave_best(best);
-        if (tid == 0) __hip_atomic_store(&p.counters[row], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) __hip_atomic_store(&p.counters[(long long)row * kRowCounterStride], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else {
         store();
     }

@@ -57,13 +57,18 @@ struct PagedAppendParams {
 };
 hipError_t launch_paged_append(const PagedAppendParams& p, const PagedBatch& b, hipStream_t s);
 
+// Words from one arrival counter to the next.  Device-scope atomics on one line of
+// memory take about 0.11 us each, one after the other: next to each other, the
+// counters of 1024 work items kept a launch of 8 x 16384 positions to 110 us.
+constexpr int kCounterStride = 64;
+
 struct PagedAttentionParams {
     PagedPool pool;
     const float* q;  // [total tokens][n_head][64]
     float* out;
     const float2* rope;
     float* part;     // softmax states of workgroups that share rows, by work item
-    int* counters;   // and their arrivals, by the rows' first work item; zero between launches
+    int* counters;   // and their arrivals, by the rows' first work item, kCounterStride apart; zero between launches
     int n_seq;
     int n_head;
     int n_head_kv;
@@ -80,6 +85,7 @@ struct PagedAttentionParams {
 // (paged_chunk_kernel).
 constexpr int kStreamRows = 16;
 constexpr int kStreamTile = 32;  // keys per tile of one wave
+constexpr int kMaxStreamParts = 128;  // work items that share a row
 constexpr int kChunkRows = 128;  // query rows of a workgroup
 struct PagedPlan {
     PagedBatch batch;  // pos and tok set by the caller

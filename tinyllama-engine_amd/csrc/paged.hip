@@ -442,13 +442,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     __shared__ int s_last;
     const int item = blockIdx.x;
     const int rank = rank_of(b, p.n_seq, item), seq = b.id(rank);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kWave - 1);
     const int local = item - b.first[rank];
     const int kvh = local % p.n_head_kv, split = local / p.n_head_kv;
     const int n_split = (b.first[rank + 1] - b.first[rank]) / p.n_head_kv;
     const int pos = b.pos[seq], n_tok = b.tok[seq + 1] - b.tok[seq];
     const int len = pos + n_tok, n_rows = n_tok * p.gqa;
     const int n_tiles = (len + kStreamTile - 1) / kStreamTile;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kWave - 1);
     const int c = lane & 15, g = lane >> 4;
     const int* const table = p.pool.table + (long long)seq * p.pool.table_stride;
     const int kv_dim = p.n_head_kv * kHeadDim, head_off = kvh * kHeadDim;
@@ -599,47 +599,67 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     for (int r = 0; r < 4; ++r) s_o[wave][r][lane] = floatx4{o[0][r], o[1][r], o[2][r], o[3][r]};
     s_ml[wave][lane] = make_float2(m_run, l_run);
     __syncthreads();
+    const auto weight = [](float m, float m_new) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new); };
+    m_run = fmaxf(fmaxf(s_ml[0][lane].x, s_ml[1][lane].x), fmaxf(s_ml[2][lane].x, s_ml[3][lane].x));
+    l_run = 0.f;
     floatx4 acc = {};
-    const auto merge = [&](int n, auto&& ml_of, auto&& o_of) {
-        float m_new = -INFINITY;
-        for (int i = 0; i < n; ++i) m_new = fmaxf(m_new, ml_of(i).x);
-        m_run = m_new;
-        l_run = 0.f;
-        acc = floatx4{};
-        for (int i = 0; i < n; ++i) {
-            const float2 ml = ml_of(i);
-            const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m_new);
-            l_run = fmaf(ml.y, f, l_run);
-            acc += o_of(i) * f;
-        }
-    };
-    merge(4, [&](int i) { return s_ml[i][lane]; }, [&](int i) { return s_o[i][wave][lane]; });
-    if (n_split > 1) {
-        const auto part_of = [&](int s) {
-            return __builtin_amdgcn_make_buffer_rsrc(
-                p.part + (long long)(b.first[rank] + s * p.n_head_kv + kvh) * (kStreamStateBytes / 4), 0, kStreamStateBytes,
-                kRawBufferWord3);
-        };
-        const auto mine = part_of(split);
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, acc), mine, 1024 * wave + 16 * lane, 0, kDeviceScope);
-        if (wave == 0)
-            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uintx2, make_float2(m_run, l_run)), mine, 4096 + 8 * lane, 0,
-                                                  kDeviceScope);
-        if (!last_to_arrive(p.counters + b.first[rank] + kvh, n_split, s_last)) return;
-        merge(n_split,
-              [&](int i) {
-                  return __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_of(i), 4096 + 8 * lane, 0, kDeviceScope));
-              },
-              [&](int i) {
-                  return __builtin_bit_cast(floatx4,
-                                            __builtin_amdgcn_raw_buffer_load_b128(part_of(i), 1024 * wave + 16 * lane, 0, kDeviceScope));
-              });
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = weight(s_ml[w][lane].x, m_run);
+        l_run = fmaf(s_ml[w][lane].y, f, l_run);
+        acc += s_o[w][wave][lane] * f;
     }
     const bool real = c < n_rows;
-    const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-    acc *= inv;
-    const bool bad = real && (not_finite(l_run) || not_finite(acc[0]) || not_finite(acc[1]) || not_finite(acc[2]) || not_finite(acc[3]));
-    if (bad) s_bad[c] = 1;
+    if (n_split > 1) {
+        // Parts in order.  A CU's device-scope loads bring about 14 GB/s here: only
+        // real rows' are made, and each max and sum is read by one lane, into the
+        // LDS that the waves' states leave.
+        const unsigned stride = p.n_head_kv * kStreamStateBytes;  // from part to part
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc(p.part + (long long)(b.first[rank] + kvh) * (kStreamStateBytes / 4), 0,
+                                                          n_split * stride, kRawBufferWord3);
+        const unsigned o_at = 1024 * wave + 16 * lane, ml_at = 4096;
+        if (real) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, acc), rs, o_at, split * stride, kDeviceScope);
+            if (wave == 0 && g == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uintx2, make_float2(m_run, l_run)), rs, ml_at + 8 * c,
+                                                      split * stride, kDeviceScope);
+        }
+        if (!last_to_arrive(p.counters + (long long)(b.first[rank] + kvh) * kCounterStride, n_split, s_last)) return;
+        float2* const s_part = reinterpret_cast<float2*>(s_o);  // [n_split][16]
+        static_assert(sizeof(s_o) >= kMaxStreamParts * 16 * sizeof(float2), "the parts' max and sum");
+        for (int i = threadIdx.x; i < 16 * n_split; i += 256)
+            if ((i & 15) < n_rows)
+                s_part[i] = __builtin_bit_cast(
+                    float2, __builtin_amdgcn_raw_buffer_load_b64(rs, (i >> 4) * stride + ml_at + 8 * (i & 15), 0, kDeviceScope));
+        __syncthreads();
+        acc = floatx4{};
+        if (real) {
+            m_run = -INFINITY;
+            for (int s = 0; s < n_split; ++s) m_run = fmaxf(m_run, s_part[16 * s + c].x);
+            l_run = 0.f;
+            constexpr int kBatch = 8;
+#pragma unroll 1
+            for (int s0 = 0; s0 < n_split; s0 += kBatch) {
+                floatx4 x[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j)
+                    if (s0 + j < n_split)
+                        x[j] = __builtin_bit_cast(
+                            floatx4, __builtin_amdgcn_raw_buffer_load_b128(rs, o_at, (s0 + j) * stride, kDeviceScope));
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j)
+                    if (s0 + j < n_split) {
+                        const float2 ml = s_part[16 * (s0 + j) + c];
+                        const float f = weight(ml.x, m_run);
+                        l_run = fmaf(ml.y, f, l_run);
+                        acc += x[j] * f;
+                    }
+            }
+        }
+    }
+    acc *= l_run == 0.f ? 0.f : 1.f / l_run;
+    if (real && (not_finite(l_run) || not_finite(acc[0]) || not_finite(acc[1]) || not_finite(acc[2]) || not_finite(acc[3])))
+        s_bad[c] = 1;
     __syncthreads();  // the row as a whole: its query may lie where its output goes
     if (real && !s_bad[c]) stg4(p.out + q_at + 16 * g + 4 * wave, make_float4(acc[0], acc[1], acc[2], acc[3]));
     // Rows that met something infinite or NaN, seen or not, once more in plain fp32.
@@ -970,7 +990,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, x), mine, 1024 * i + 16 * lane, 0, kDeviceScope);
         }
         __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uintx2, make_float2(m_run, l_run)), mine, 8192 + 8 * lane, 0, kDeviceScope);
-        if (!last_to_arrive(p.counters + b.first[rank] + (n_rt - 1 - rt) * n_combo + kvh, n_split, s_last)) return;
+        if (!last_to_arrive(p.counters + (long long)(b.first[rank] + (n_rt - 1 - rt) * n_combo + kvh) * kCounterStride, n_split, s_last)) return;
         m_run = -INFINITY;
         l_run = 0.f;
         o[0] = o[1] = floatx16{};

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "paged.h"
 
@@ -35,7 +36,9 @@ inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, PagedPlan* 
         tiles[s] = n_tok > 0 && n_tok * gqa <= kStreamRows ? (b.pos[s] + n_tok + kStreamTile - 1) / kStreamTile : 0;
         most = std::max(most, tiles[s]);
     }
-    const int part = part_tiles(4, most, 4ll * n_cu, [&](int len) {
+    const char* sl = getenv("SL"); const int slots = sl ? atoi(sl) : 4;
+    const int least = std::max(getenv("LE") ? atoi(getenv("LE")) : 4, (most + kMaxStreamParts - 1) / kMaxStreamParts);
+    const int part = part_tiles(least, most, (long long)slots * n_cu, [&](int len) {
         long long n = 0;
         for (int s = 0; s < n_seq; ++s) n += (tiles[s] + len - 1) / len;
         return n * n_head_kv;
