@@ -41,7 +41,7 @@ int main()
             if (chunk)
                 plan_chunk(n_seq, hkv, gqa, n_cu, type, plan.get());
             else
-                plan_stream(n_seq, hkv, gqa, n_cu, plan.get());
+                plan_stream(n_seq, hkv, gqa, n_cu, type, plan.get());
             if (plan->n_items == 0) continue;
             CHECK(plan->n_items == b.first[n_seq] && b.first[0] == 0);
             bool shared = false;

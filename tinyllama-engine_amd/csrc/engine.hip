@@ -1419,7 +1419,7 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
         if (chunk)
             plan_chunk(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &plan);
         else
-            plan_stream(n_seq, p.n_head_kv, p.gqa, e->n_cu, &plan);
+            plan_stream(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &plan);
         if (plan.n_items == 0) continue;
         if (plan.shared) {
             const size_t items = static_cast<size_t>(plan.n_items);

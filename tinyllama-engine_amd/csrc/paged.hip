@@ -594,22 +594,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     }
     l_run = sum_xor32(sum_xor16(l_run));  // the lane groups summed different keys
 
-    // The four waves' states meet: wave w goes on with dimensions 16 g + 4 w .. + 3.
+    // The waves' states meet: wave w goes on with dimensions 16 g + 4 w .. + 3.
 #pragma unroll
     for (int r = 0; r < 4; ++r) s_o[wave][r][lane] = floatx4{o[0][r], o[1][r], o[2][r], o[3][r]};
     s_ml[wave][lane] = make_float2(m_run, l_run);
     __syncthreads();
     const auto weight = [](float m, float m_new) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new); };
+    const bool real = c < n_rows;
+    floatx4 acc = {};
     m_run = fmaxf(fmaxf(s_ml[0][lane].x, s_ml[1][lane].x), fmaxf(s_ml[2][lane].x, s_ml[3][lane].x));
     l_run = 0.f;
-    floatx4 acc = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         const float f = weight(s_ml[w][lane].x, m_run);
         l_run = fmaf(s_ml[w][lane].y, f, l_run);
         acc += s_o[w][wave][lane] * f;
     }
-    const bool real = c < n_rows;
     if (n_split > 1) {
         // Parts in order.  A CU's device-scope loads bring about 14 GB/s here: only
         // real rows' are made, and each max and sum is read by one lane, into the

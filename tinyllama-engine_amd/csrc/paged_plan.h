@@ -2,53 +2,63 @@
 #pragma once
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "paged.h"
 
 namespace tla {
 
-// The smallest part length from `least` to `most` tiles with which the units
-// (items_at(length) work items) are at most `slots`, as many as run at once;
-// `most` if there are more even so.
-template <class F>
-inline int part_tiles(int least, int most, long long slots, F&& items_at)
-{
-    int lo = least, hi = std::max(least, most);
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (items_at(mid) <= slots)
-            hi = mid;
-        else
-            lo = mid + 1;
-    }
-    return lo;
-}
-
-// Parts of at least one tile per wave, such that the launch is one round of
-// four workgroups per CU if it can be.
-inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, PagedPlan* p)
+// Parts of the keys by estimated time in us, fitted to launches of 1 to 200
+// sequences of 128 to 16384 positions, 32 / 4 heads (F16, one sequence of 16384
+// positions in 16 / 32 / 64 / 128 parts 15.5 / 14.1 / 17.1 / 26.6 us; 64 of 1100
+// whole / in halves 15.9 / 18.6; 64 of 255 to 2047 whole / by 32 / 21 / 16 tiles
+// 24.3 / 21.4 / 20.9 / 20.8; F32, 8 of 16384 in 6 / 8 / 16 / 32 parts 59.9 / 55.6 /
+// 56.9 / 59.8): all tiles at the rate of memory, less with fewer work items than
+// CUs, or the longest part's steps of a wave if that is longer; an uneven end, the
+// less the more items a CU has; handing over, and adding one part after the other;
+// each further round of four workgroups per CU (96 of 125 to 1000 in 1080 / 700
+// items 21.1 / 17.2).
+inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* p)
 {
     PagedBatch& b = p->batch;
+    const double memory = (type == kKvF32 ? 2.6e-3 : 1.3e-3) * 256 / n_cu, step = type == kKvF32 ? 0.4 : 0.19;
     int tiles[kMaxSeqPerLaunch], most = 0;
+    double total = 0;
     for (int s = 0; s < n_seq; ++s) {
         const int n_tok = b.tok[s + 1] - b.tok[s];
         tiles[s] = n_tok > 0 && n_tok * gqa <= kStreamRows ? (b.pos[s] + n_tok + kStreamTile - 1) / kStreamTile : 0;
         most = std::max(most, tiles[s]);
+        total += tiles[s];
     }
-    const char* sl = getenv("SL"); const int slots = sl ? atoi(sl) : 4;
-    const int least = std::max(getenv("LE") ? atoi(getenv("LE")) : 4, (most + kMaxStreamParts - 1) / kMaxStreamParts);
-    const int part = part_tiles(least, most, (long long)slots * n_cu, [&](int len) {
-        long long n = 0;
-        for (int s = 0; s < n_seq; ++s) n += (tiles[s] + len - 1) / len;
-        return n * n_head_kv;
-    });
+    p->n_items = 0;
     p->shared = false;
+    if (!most) return;
+    p->split_tiles = most;
+    double best = 0;
+    int worse = 0;
+    for (const int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
+        static_assert(kMaxStreamParts == 128);
+        const int len = (most + parts - 1) / parts;
+        if (parts > 1 && (len < 4 || worse > 3)) break;  // a tile for each wave
+        long long items = 0;
+        for (int s = 0; s < n_seq; ++s) items += (tiles[s] + len - 1) / len;
+        items *= n_head_kv;
+        const double per_item = static_cast<double>(n_cu) / items;  // CUs
+        const double us = std::max(total * n_head_kv * memory * std::max(1.0, per_item), len * step) +
+                          (total * n_head_kv < 0.8 * len * items ? 0.14 * len * std::min(1.0, per_item) : 0) +
+                          (parts > 1 ? 2.2 + 0.15 * parts : 0) + 3.0 * ((items - 1) / (4 * n_cu));
+        if (parts == 1 || us < best) {
+            best = us;
+            p->split_tiles = len;
+            worse = 0;
+        } else {
+            ++worse;
+        }
+    }
     long long at = 0;
     for (int s = 0; s < n_seq; ++s) {
         b.first[s] = static_cast<int>(at);
         b.set_id(s, s);
-        const int n = (tiles[s] + part - 1) / part;
+        const int n = (tiles[s] + p->split_tiles - 1) / p->split_tiles;
         p->shared |= n > 1;
         at += static_cast<long long>(n) * n_head_kv;
     }
