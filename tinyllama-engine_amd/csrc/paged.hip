@@ -203,9 +203,18 @@ struct Pieces<kKvF16> {
     static __device__ __forceinline__ void split(floatx8 v, Frag (&o)[kN])
     {
         o[0] = __builtin_convertvector(v, f16x8);
-        floatx8 r;  // exact; one v_fma_mix each
+        // v - o[0], exact, by the mixed fma, which reads either half of a word as
+        // an F16: half the operations of widening and subtracting.
+        const uintx4 w = __builtin_bit_cast(uintx4, o[0]);
+        floatx8 r;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] = fmaf((float)o[0][e], -1.f, v[e]);
+        for (int i = 0; i < 4; ++i) {
+            float lo, hi;
+            asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(w[i]), "v"(v[2 * i]));
+            asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(hi) : "v"(w[i]), "v"(v[2 * i + 1]));
+            r[2 * i] = lo;
+            r[2 * i + 1] = hi;
+        }
         o[1] = __builtin_convertvector(r, f16x8);
     }
     static __device__ __forceinline__ floatx4 mfma16(Frag a, Frag b, floatx4 c)
@@ -928,8 +937,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     store(0);
     __syncthreads();
     floatx16 o[2] = {};
-    float m_run = -INFINITY, l_run = 0.f;
+    // Probabilities are 2^(s + off), off = kShift - m_run.  m_run is a row's largest
+    // score of some tile, -inf before its first key; it is looked for again when
+    // the sum of a lane's 16 probabilities passes kLimit: most tiles form no
+    // maximum and do not rescale O.  The scores are then formed once more (kAgain):
+    // 16 registers fewer are live.  Not for F32, whose products are 3 to 6 times as
+    // many.
+    float m_run = -INFINITY, l_run = 0.f, off = 0.f;
     constexpr float kShift = P::kShift;
+    constexpr bool kAgain = kType != kKvF32;
+    constexpr float kLimit = kType == kKvF16 ? 16384.f : 256.f;
     for (int tile = tile0; tile < tile_end; ++tile) {
         const int buf = (tile - tile0) & 1;
         if (tile + 1 < tile_end) {
@@ -941,35 +958,50 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
             const int key = tile * kKeys + 32 * u;
             const unsigned seen = __builtin_amdgcn_readfirstlane(s_there[buf][u]);
             if (key > wave_last || seen == 0) continue;  // uniform over the wave
-            floatx16 s = Tile::scores(s_kv[buf][u], q, lane);
-            if (key + 31 > wave_first || seen != ~0u) {
+            const auto scores = [&] {
+                floatx16 s = Tile::scores(s_kv[buf][u], q, lane);
+                if (key + 31 > wave_first || seen != ~0u) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = 16 * (r >> 3) + 8 * half + (r & 7);
+                        s[r] = key + j <= qpos && (seen >> j & 1) ? s[r] : -INFINITY;
+                    }
+                }
+                return s;
+            };
+            float sum;
+            const auto weights = [&](floatx16 s) {
+                sum = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int j = 16 * (r >> 3) + 8 * half + (r & 7);
-                    s[r] = key + j <= qpos && (seen >> j & 1) ? s[r] : -INFINITY;
+                    s[r] = __builtin_amdgcn_exp2f(P::kScaled ? fmaf(s[r], down, off) : s[r] + off);
+                    sum += s[r];
                 }
-            }
-            float mx = s[0];
+                return s;
+            };
+            const floatx16 first = scores();
+            floatx16 e = weights(first);
+            if (__any(m_run == -INFINITY || sum > kLimit)) {
+                floatx16 s;
+                if constexpr (kAgain)
+                    s = scores();
+                else
+                    s = first;
+                float mx = s[0];
 #pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-            mx = max_xor32(mx) * down;
-            if (__any(mx > m_run + kRescaleSlack)) {
-                const float m_new = fmaxf(m_run, mx);
-                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+                const float m_new = fmaxf(m_run, max_xor32(mx) * down);
+                // a row that has seen nothing yet keeps its offset of 0
+                off = m_new == -INFINITY ? 0.f : kShift - m_new;
+                const float alpha = m_run == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
                 m_run = m_new;
                 l_run *= alpha;
                 o[0] *= alpha;
                 o[1] *= alpha;
-            }
-            const float m_use = m_run == -INFINITY ? 0.f : m_run - kShift;
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], down, -m_use));
-                sum += s[r];
+                e = weights(s);
             }
             l_run += sum;
-            Tile::accumulate(s, s_kv[buf][u], lane, o);
+            Tile::accumulate(e, s_kv[buf][u], lane, o);
         }
         if (tile + 1 < tile_end) store(buf ^ 1);  // read before the barrier that ended the last step
         __syncthreads();
