@@ -278,6 +278,15 @@ __device__ __forceinline__ bool not_finite(float x)
     return !(__builtin_fabsf(x) <= 3.4028234663852886e38f);
 }
 
+// A word of a page table at a place that is the same for the whole wave, by a
+// scalar load.  (Next to loads into LDS the compiler takes the table for memory
+// that they may change, reads it through the vector cache, and waits for them.)
+__device__ __forceinline__ int page_at(const int* table, int at)
+{
+    typedef const int __attribute__((address_space(4))) * Constant;
+    return ((Constant)(uintptr_t)table)[at];
+}
+
 // Up to 16 rows of 64 elements of one kv head from one page, as a buffer
 // whose range ends with them: loads past the last row, and all of an absent
 // page's, give zeros without touching memory.
@@ -479,7 +488,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     const auto look_up = [&](int tile) {
         if constexpr (!kSmall) {
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) page[hf] = table[min(tile * kStreamTile + 16 * hf, len - 1) >> p.pool.page_shift];
+            for (int hf = 0; hf < 2; ++hf) page[hf] = page_at(table, min(tile * kStreamTile + 16 * hf, len - 1) >> p.pool.page_shift);
         }
     };
     const unsigned row_bytes = kv_dim * sizeof(T);
@@ -683,91 +692,64 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
 
 // ---- chunks --------------------------------------------------------------------------
 
-// A tile's keys and values in LDS, in the order in which the 32x32 MFMA
-// operands are read: planes of 32 keys, one per piece.
-//   K plane: byte 512 c + 16 (kperm(i) ^ c) = dimensions 8 c .. + 7 of key i; kperm
-//     as in the prefill kernel makes the scores of the S accumulator the B
-//     operand of P.V, c spreads the eight pieces of a row that one load
-//     brings over the banks.
-//   V plane: byte 2048 dt + 1024 s + 512 h + 16 i = keys 16 s + 8 h .. + 7 of dimension 2 i + dt.
-constexpr int kPlane = 32 * kHeadDim * 2;
+// 32 keys and values in LDS, as the 32x32 MFMA operands are read.  Score register
+// r of lane (half, col) is key 16 (r / 8) + 8 half + r % 8 for query col, if row
+// i of the K operand is key kperm(i) (bits 2 and 3 swapped); the same registers
+// are the B operand (P^T) of P.V, whose k step s, element e of half is key 16 s +
+// 8 half + e.
+constexpr int kPlane = 32 * kHeadDim * 2;  // bytes of 32 rows of 16-bit elements
 
 __device__ __forceinline__ int kperm(int i)
 {
     return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1);
 }
 
+// 16-bit elements: K, then V, as rows of 128 bytes whose 16-byte chunks are
+// permuted, chunk c of key i at place c ^ chunk_swap(i), so that both kinds of
+// read take each bank once.  V's operand, eight keys of one dimension, is read
+// through the LDS transpose: of the 16 lanes of a group, lane 4 j + m gives the
+// address of dimensions 4 m .. of key j, and lane i receives dimension i of keys
+// 0 .. 3.  O register r of dt is dimension 32 dt + 8 (r / 4) + 4 half + r % 4.
+__device__ __forceinline__ int chunk_swap(int key)
+{
+    return key >> 1 & 7;
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4_t* lds_short4;
+
 template <int kType>
 struct ChunkTile {
     typedef Pieces<kType> P;
     typedef typename P::Frag Frag;
-    static constexpr int kCache = kType == kKvF32 ? 3 : 1;  // planes of a cache element
     static constexpr int kKeys = chunk_tile(kType);
-    static constexpr int kSub = kKeys / 32;                 // 32-key planes per tile
-    static constexpr int kBytes = 2 * kCache * kPlane;      // K and V planes of 32 keys
-    typedef std::conditional_t<kType == kKvF32, floatx8, uintx4> KRaw;                          // 8 dimensions of a key
-    typedef std::conditional_t<kType == kKvF32, floatx2, unsigned> VRaw;                        // 2 dimensions of a key
-
-    // One thread's share of 32 keys: dimensions 8 kc .. of key kk, dimensions
-    // 2 vi, 2 vi + 1 of keys 4 vg ..
-    static __device__ __forceinline__ void store(const KRaw& k, const VRaw (&v)[4], unsigned char* at, int kk, int kc,
-                                                 int vi, int vg)
+    static constexpr int kSub = kKeys / 32;  // per tile
+    static constexpr int kBytes = 2 * kPlane;
+    static __device__ __forceinline__ int dim_of(int dt, int r, int half) { return 32 * dt + 8 * (r >> 2) + 4 * half + (r & 3); }
+    // The byte of this lane's pieces: K at k step 0, V at k step 0, dt 0, keys 0 .. 3.
+    static __device__ __forceinline__ int k_at(int lane)
     {
-        const int k_at = 512 * kc + 16 * (kperm(kk) ^ kc);
-        const int v_at = 1024 * (vg >> 2) + 512 * (vg >> 1 & 1) + 16 * vi + 8 * (vg & 1);
-        if constexpr (kType == kKvF32) {
-            Frag f[3];
-            P::split(k, f);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) *reinterpret_cast<Frag*>(at + i * kPlane + k_at) = f[i];
-            floatx8 x;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = v[e & 3][e >> 2];
-            P::split(x, f);  // dt 0, then dt 1
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const uintx4 w = __builtin_bit_cast(uintx4, f[i]);
-                unsigned char* const va = at + (3 + i) * kPlane + v_at;
-                *reinterpret_cast<uintx2*>(va) = uintx2{w[0], w[1]};
-                *reinterpret_cast<uintx2*>(va + 2048) = uintx2{w[2], w[3]};
-            }
-        } else {
-            *reinterpret_cast<uintx4*>(at + k_at) = k;
-            unsigned char* const va = at + kPlane + v_at;
-            *reinterpret_cast<uintx2*>(va) = uintx2{__builtin_amdgcn_perm(v[1], v[0], 0x05040100), __builtin_amdgcn_perm(v[3], v[2], 0x05040100)};
-            *reinterpret_cast<uintx2*>(va + 2048) = uintx2{__builtin_amdgcn_perm(v[1], v[0], 0x07060302), __builtin_amdgcn_perm(v[3], v[2], 0x07060302)};
-        }
+        const int key = kperm(lane & 31);
+        return 128 * key + 16 * ((lane >> 5) ^ chunk_swap(key));
     }
-    static __device__ __forceinline__ floatx16 products(const Frag (&a)[kCache], const Frag (&b)[P::kN], floatx16 c)
+    static __device__ __forceinline__ int v_at(int lane)
     {
-        if constexpr (kType == kKvF32) {
-            c = P::mfma32(a[2], b[0], c);
-            c = P::mfma32(a[1], b[1], c);
-            c = P::mfma32(a[0], b[2], c);
-            c = P::mfma32(a[1], b[0], c);
-            c = P::mfma32(a[0], b[1], c);
-            c = P::mfma32(a[0], b[0], c);
-        } else {
-#pragma unroll
-            for (int i = P::kN - 1; i >= 0; --i) c = P::mfma32(a[0], b[i], c);
-        }
-        return c;
+        const int key = 8 * (lane >> 5) + (lane >> 2 & 3), chunk = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+        return kPlane + 128 * key + 16 * (chunk ^ chunk_swap(key)) + 8 * (lane & 1);
     }
-    static __device__ __forceinline__ floatx16 scores(const unsigned char* at, const Frag (&q)[4][P::kN], int lane)
+    static __device__ __forceinline__ floatx16 scores(const unsigned char* at, const Frag (&q)[4][P::kN], int k_at)
     {
         floatx16 s = {};
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-            const int c = 2 * ks + (lane >> 5);
-            Frag a[kCache];
+            const Frag a = *reinterpret_cast<const Frag*>(at + (k_at ^ 32 * ks));
 #pragma unroll
-            for (int i = 0; i < kCache; ++i)
-                a[i] = *reinterpret_cast<const Frag*>(at + i * kPlane + 512 * c + 16 * ((lane & 31) ^ c));
-            s = products(a, q[ks], s);
+            for (int i = P::kN - 1; i >= 0; --i) s = P::mfma32(a, q[ks][i], s);
         }
         return s;
     }
-    static __device__ __forceinline__ void accumulate(const floatx16& s, const unsigned char* at, int lane, floatx16 (&o)[2])
+    static __device__ __forceinline__ void accumulate(const floatx16& s, const unsigned char* at, int v_at, floatx16 (&o)[2])
     {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -778,10 +760,96 @@ struct ChunkTile {
             P::split(pv, f);
 #pragma unroll
             for (int dt = 0; dt < 2; ++dt) {
-                Frag a[kCache];
+                struct {
+                    short4_t x[2];
+                } w;
 #pragma unroll
-                for (int i = 0; i < kCache; ++i)
-                    a[i] = *reinterpret_cast<const Frag*>(at + (kCache + i) * kPlane + 2048 * dt + 1024 * ks + 16 * lane);
+                for (int h = 0; h < 2; ++h)  // keys 4 h .. + 3: chunk_swap is 2 h further
+                    w.x[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_short4)(at + (v_at ^ 32 * h ^ 64 * dt) + 512 * h + 2048 * ks));
+                const Frag a = __builtin_bit_cast(Frag, w);
+#pragma unroll
+                for (int i = P::kN - 1; i >= 0; --i) o[dt] = P::mfma32(a, f[i], o[dt]);
+            }
+        }
+    }
+};
+
+// F32 elements, split into three planes each when a tile arrives.
+//   K plane: byte 512 c + 16 (kperm(i) ^ c) = dimensions 8 c .. + 7 of key i (c spreads
+//     the eight pieces of a row that one load brings over the banks).
+//   V plane: byte 2048 dt + 1024 s + 512 h + 16 i = keys 16 s + 8 h .. + 7 of dimension 2 i + dt.
+template <>
+struct ChunkTile<kKvF32> {
+    typedef Pieces<kKvF32> P;
+    typedef P::Frag Frag;
+    static constexpr int kKeys = chunk_tile(kKvF32);
+    static constexpr int kSub = kKeys / 32;
+    static constexpr int kBytes = 6 * kPlane;
+    static __device__ __forceinline__ int dim_of(int dt, int r, int half) { return 16 * (r >> 2) + 8 * half + 2 * (r & 3) + dt; }
+    static __device__ __forceinline__ int k_at(int lane) { return lane; }
+    static __device__ __forceinline__ int v_at(int lane) { return 3 * kPlane + 16 * lane; }
+    // One thread's share of 32 keys: dimensions 8 kc .. of key kk, dimensions
+    // 2 vi, 2 vi + 1 of keys 4 vg ..
+    static __device__ __forceinline__ void store(const floatx8& k, const floatx2 (&v)[4], unsigned char* at, int kk, int kc,
+                                                 int vi, int vg)
+    {
+        Frag f[3];
+        P::split(k, f);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) *reinterpret_cast<Frag*>(at + i * kPlane + 512 * kc + 16 * (kperm(kk) ^ kc)) = f[i];
+        floatx8 x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = v[e & 3][e >> 2];
+        P::split(x, f);  // dt 0, then dt 1
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const uintx4 w = __builtin_bit_cast(uintx4, f[i]);
+            unsigned char* const va = at + (3 + i) * kPlane + 1024 * (vg >> 2) + 512 * (vg >> 1 & 1) + 16 * vi + 8 * (vg & 1);
+            *reinterpret_cast<uintx2*>(va) = uintx2{w[0], w[1]};
+            *reinterpret_cast<uintx2*>(va + 2048) = uintx2{w[2], w[3]};
+        }
+    }
+    // The six products of pieces, small ones first.
+    static __device__ __forceinline__ floatx16 products(const Frag (&a)[3], const Frag (&b)[3], floatx16 c)
+    {
+        c = P::mfma32(a[2], b[0], c);
+        c = P::mfma32(a[1], b[1], c);
+        c = P::mfma32(a[0], b[2], c);
+        c = P::mfma32(a[1], b[0], c);
+        c = P::mfma32(a[0], b[1], c);
+        c = P::mfma32(a[0], b[0], c);
+        return c;
+    }
+    static __device__ __forceinline__ floatx16 scores(const unsigned char* at, const Frag (&q)[4][3], int lane)
+    {
+        floatx16 s = {};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const int c = 2 * ks + (lane >> 5);
+            Frag a[3];
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                a[i] = *reinterpret_cast<const Frag*>(at + i * kPlane + 512 * c + 16 * ((lane & 31) ^ c));
+            s = products(a, q[ks], s);
+        }
+        return s;
+    }
+    static __device__ __forceinline__ void accumulate(const floatx16& s, const unsigned char* at, int v_at, floatx16 (&o)[2])
+    {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            floatx8 pv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pv[e] = s[8 * ks + e];
+            Frag f[3];
+            P::split(pv, f);
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt) {
+                Frag a[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    a[i] = *reinterpret_cast<const Frag*>(at + i * kPlane + 2048 * dt + 1024 * ks + v_at);
                 o[dt] = products(a, f, o[dt]);
             }
         }
@@ -790,8 +858,9 @@ struct ChunkTile {
 
 // Rows of one sequence and kv head, 128 of them: (token, head) pairs in order,
 // 32 to a wave.  A work item is such a tile of rows over a range of key tiles;
-// its waves share the tiles in LDS, double-buffered, the next one's rows
-// on their way in registers while the waves compute.
+// its waves share the tiles in LDS, double-buffered: the next one's rows are on
+// their way while the waves compute, directly into LDS (16-bit elements of large
+// pages) or in registers.
 // kSmall: pages of fewer than 8 positions, whose rows are looked up by each
 // lane; else the eight rows that a wave loads lie in one page.
 template <int kType, bool kSmall, int kMaxSeq>
@@ -827,33 +896,45 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     const int col = lane & 31, half = lane >> 5;
     const int* const table = p.pool.table + (long long)seq * p.pool.table_stride;
     const int kv_dim = p.n_head_kv * kHeadDim, head_off = kvh * kHeadDim;
-    const int kk = threadIdx.x >> 3, kc = threadIdx.x & 7;   // this thread's piece of K
-    const int vg = threadIdx.x >> 5, vi = threadIdx.x & 31;  // and of V
-
-    typename Tile::KRaw k_raw[kSub];
-    typename Tile::VRaw v_raw[kSub][4];
-    unsigned there[kSub];  // the wave's eight rows
+    // This thread's piece of 32 keys.  F32: eight dimensions of key kk, and two of
+    // four keys' values; else 16 bytes of key kk and of its values: chunk kc's place.
+    constexpr bool kF32 = kType == kKvF32, kDirect = !kF32 && !kSmall;
+    const int kk = threadIdx.x >> 3, kc = threadIdx.x & 7;
+    const int vg = threadIdx.x >> 5, vi = threadIdx.x & 31;
+    const int chunk = kF32 ? kc : kc ^ chunk_swap(kk);
+    typedef std::conditional_t<kF32, floatx8, uintx4> KRaw;
+    KRaw k_raw[kSub];
+    uintx4 w_raw[kSub];       // values: 16-bit
+    floatx2 v_raw[kSub][4];   // F32
+    unsigned there[kSub];     // the wave's eight rows
     int page[kSub];
+    const unsigned row_bytes = kv_dim * sizeof(T);
+    const unsigned k_off = (kk & 7) * row_bytes + 8 * chunk * sizeof(T), v_off = 4 * (vg & 1) * row_bytes + 2 * vi * sizeof(T);
     const auto look_up = [&](int tile) {
         if constexpr (!kSmall) {
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) page[u] = table[min(tile * kKeys + 32 * u + 8 * wave, len - 1) >> p.pool.page_shift];
+            for (int u = 0; u < kSub; ++u) page[u] = page_at(table, min(tile * kKeys + 32 * u + 8 * wave, len - 1) >> p.pool.page_shift);
         }
     };
-    const auto load = [&](int tile) {
+    // Requests a tile's rows: into registers, or (kDirect) into LDS buffer buf.
+    const auto load = [&](int tile, int buf) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
             const int key = tile * kKeys + 32 * u + 8 * wave;  // the wave's first
             if constexpr (kSmall) {
                 const auto at = [&](int j) { return j < len ? row_of(p.pool, table, j, kv_dim) : -1; };
                 const long long kr = at(tile * kKeys + 32 * u + kk);
-                const T* const ka = static_cast<const T*>(p.pool.k) + kr + head_off + 8 * kc;
-                k_raw[u] = kr >= 0 ? *reinterpret_cast<const typename Tile::KRaw*>(ka) : typename Tile::KRaw{};
+                const long long k_el = kr + head_off + 8 * chunk;
+                k_raw[u] = kr >= 0 ? *reinterpret_cast<const KRaw*>(static_cast<const T*>(p.pool.k) + k_el) : KRaw{};
+                if constexpr (kF32) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const long long vr = at(tile * kKeys + 32 * u + 4 * vg + e);
-                    const T* const va = static_cast<const T*>(p.pool.v) + vr + head_off + 2 * vi;
-                    v_raw[u][e] = vr >= 0 ? *reinterpret_cast<const typename Tile::VRaw*>(va) : typename Tile::VRaw{};
+                    for (int e = 0; e < 4; ++e) {
+                        const long long vr = at(tile * kKeys + 32 * u + 4 * vg + e);
+                        const T* const va = static_cast<const T*>(p.pool.v) + vr + head_off + 2 * vi;
+                        v_raw[u][e] = vr >= 0 ? *reinterpret_cast<const floatx2*>(va) : floatx2{};
+                    }
+                } else {
+                    w_raw[u] = kr >= 0 ? *reinterpret_cast<const uintx4*>(static_cast<const T*>(p.pool.v) + k_el) : uintx4{};
                 }
                 const unsigned long long m = __ballot(kr >= 0);  // eight lanes to a key
                 there[u] = 0;
@@ -864,41 +945,50 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
                 const long long at = seen ? (long long)page[u] * p.pool.page_stride +
                                                 (long long)(key & ((1 << p.pool.page_shift) - 1)) * kv_dim + head_off
                                           : 0;
-                const unsigned row_bytes = kv_dim * sizeof(T);
-                const int rows = min(8, len - key);
-                const unsigned bytes = seen ? (rows - 1) * row_bytes + kHeadDim * (unsigned)sizeof(T) : 0;
+                const unsigned bytes = seen ? (min(8, len - key) - 1) * row_bytes + kHeadDim * (unsigned)sizeof(T) : 0;
                 const auto rk = rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(p.pool.k) + at), bytes});
                 const auto rv = rsrc_of({reinterpret_cast<const char*>(static_cast<const T*>(p.pool.v) + at), bytes});
-                const unsigned ko = (kk & 7) * row_bytes + 8 * kc * sizeof(T);
-                if constexpr (kType == kKvF32) {
-                    const floatx4 x = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko, 0, 0));
-                    const floatx4 y = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko + 16, 0, 0));
+                if constexpr (kF32) {
+                    const floatx4 x = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off, 0, 0));
+                    const floatx4 y = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + 16, 0, 0));
                     k_raw[u] = floatx8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-                } else {
-                    k_raw[u] = __builtin_amdgcn_raw_buffer_load_b128(rk, ko, 0, 0);
-                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const unsigned vo = (4 * (vg & 1) + e) * row_bytes + 2 * vi * sizeof(T);
-                    if constexpr (kType == kKvF32)
-                        v_raw[u][e] = __builtin_bit_cast(floatx2, __builtin_amdgcn_raw_buffer_load_b64(rv, vo, 0, 0));
-                    else
-                        v_raw[u][e] = __builtin_amdgcn_raw_buffer_load_b32(rv, vo, 0, 0);
+                    for (int e = 0; e < 4; ++e)
+                        v_raw[u][e] = __builtin_bit_cast(floatx2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_off + e * row_bytes, 0, 0));
+                } else {  // lane l's 16 bytes land at byte 16 l of the wave's KiB
+                    unsigned char* const to = s_kv[buf][u] + 1024 * wave;
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)to, 16, k_off, 0, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(to + kPlane), 16, k_off, 0, 0, 0);
                 }
                 there[u] = seen ? 255 : 0;
             }
+            if constexpr (kDirect)
+                if (lane == 0) reinterpret_cast<unsigned char*>(&s_there[buf][u])[wave] = (unsigned char)there[u];
         }
     };
+    // Puts the tile requested last into LDS buffer buf, or waits until it is there.
     const auto store = [&](int buf) {
+        if constexpr (kDirect) {
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0)
+        } else {
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-            Tile::store(k_raw[u], v_raw[u], s_kv[buf][u], kk, kc, vi, vg);
-            if (lane == 0) reinterpret_cast<unsigned char*>(&s_there[buf][u])[wave] = (unsigned char)there[u];
+            for (int u = 0; u < kSub; ++u) {
+                if constexpr (kF32) {
+                    Tile::store(k_raw[u], v_raw[u], s_kv[buf][u], kk, kc, vi, vg);
+                } else {
+                    unsigned char* const to = s_kv[buf][u] + 128 * kk + 16 * kc;
+                    *reinterpret_cast<uintx4*>(to) = k_raw[u];
+                    *reinterpret_cast<uintx4*>(to + kPlane) = w_raw[u];
+                }
+                if (lane == 0) reinterpret_cast<unsigned char*>(&s_there[buf][u])[wave] = (unsigned char)there[u];
+            }
         }
     };
+    const int k_at = Tile::k_at(lane), v_at = Tile::v_at(lane);
 
     look_up(tile0);
-    load(tile0);
+    load(tile0, 0);
     look_up(min(tile0 + 1, n_tiles - 1));
 
     // The row's query: lane (half, col) holds dimensions 16 s + 8 half .. + 7 for k step s.
@@ -950,7 +1040,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     for (int tile = tile0; tile < tile_end; ++tile) {
         const int buf = (tile - tile0) & 1;
         if (tile + 1 < tile_end) {
-            load(tile + 1);
+            load(tile + 1, buf ^ 1);  // read before the barrier that ended the last step
             look_up(min(tile + 2, n_tiles - 1));
         }
 #pragma unroll
@@ -959,7 +1049,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
             const unsigned seen = __builtin_amdgcn_readfirstlane(s_there[buf][u]);
             if (key > wave_last || seen == 0) continue;  // uniform over the wave
             const auto scores = [&] {
-                floatx16 s = Tile::scores(s_kv[buf][u], q, lane);
+                floatx16 s = Tile::scores(s_kv[buf][u], q, k_at);
                 if (key + 31 > wave_first || seen != ~0u) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
@@ -1001,9 +1091,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
                 e = weights(s);
             }
             l_run += sum;
-            Tile::accumulate(e, s_kv[buf][u], lane, o);
+            Tile::accumulate(e, s_kv[buf][u], v_at, o);
         }
-        if (tile + 1 < tile_end) store(buf ^ 1);  // read before the barrier that ended the last step
+        if (tile + 1 < tile_end) store(buf ^ 1);
         __syncthreads();
     }
     l_run = sum_xor32(l_run);
@@ -1056,12 +1146,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     // The row as a whole: its query may lie where its output goes.
     const unsigned long long bads = __ballot(real && bad);
     const unsigned bad_rows = (unsigned)bads | (unsigned)(bads >> 32);
-    if (real && !(bad_rows >> col & 1)) {  // o[dt][4 a + e] = dimension 16 a + 8 half + 2 e + dt
-        float* const orow = p.out + q_at + 8 * half;
+    if (real && !(bad_rows >> col & 1)) {
+        float* const orow = p.out + q_at;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-            stg4(orow + 16 * a, make_float4(o[0][4 * a], o[1][4 * a], o[0][4 * a + 1], o[1][4 * a + 1]));
-            stg4(orow + 16 * a + 4, make_float4(o[0][4 * a + 2], o[1][4 * a + 2], o[0][4 * a + 3], o[1][4 * a + 3]));
+            if constexpr (kF32) {  // two dt side by side
+                float* const to = orow + Tile::dim_of(0, 4 * a, half);
+                stg4(to, make_float4(o[0][4 * a], o[1][4 * a], o[0][4 * a + 1], o[1][4 * a + 1]));
+                stg4(to + 4, make_float4(o[0][4 * a + 2], o[1][4 * a + 2], o[0][4 * a + 3], o[1][4 * a + 3]));
+            } else {
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt)
+                    stg4(orow + Tile::dim_of(dt, 4 * a, half),
+                         make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]));
+            }
         }
     }
     // Rows that met something infinite or NaN, seen or not, once more in plain fp32.
