@@ -265,12 +265,25 @@ __device__ __forceinline__ float4 rotate4_fma(float4 x, float4 cs)
                        __builtin_fmaf(x.z, cs.z, -(x.w * cs.w)), __builtin_fmaf(x.z, cs.w, x.w * cs.z));
 }
 
-__device__ __forceinline__ floatx4 scaled_q4(const float* q, const float* cs, int d, int rotate, float scale)
+// kN pieces of four dimensions of a query row, dim(i) .., scaled and, if asked,
+// rotated.  All loads are issued before any is used, the (cos, sin) also where they
+// are not needed: with a branch for them each piece waits for its loads in turn
+// (16 times 0.6 us in a chunk's workgroup).
+template <int kN, class F>
+__device__ __forceinline__ void load_q(const float* q, const float* cs, F&& dim, int rotate, float scale, floatx4 (&x)[kN])
 {
-    float4 x = ldg4(q + d);
-    x = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
-    if (rotate) x = rotate4_fma(x, ldg4(cs + d));
-    return floatx4{x.x, x.y, x.z, x.w};
+    float4 v[kN], r[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        v[i] = ldg4(q + dim(i));
+        r[i] = ldg4(cs + dim(i));
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        const float4 s = make_float4(v[i].x * scale, v[i].y * scale, v[i].z * scale, v[i].w * scale);
+        const float4 t = rotate4_fma(s, r[i]);
+        x[i] = rotate ? floatx4{t.x, t.y, t.z, t.w} : floatx4{s.x, s.y, s.z, s.w};
+    }
 }
 
 __device__ __forceinline__ bool not_finite(float x)
@@ -558,8 +571,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     typename Tile::Query q;
     {
         floatx4 x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = scaled_q4(p.q + q_at, cs, Tile::q_dim(i, g), p.rotate, p.scale_log2);
+        load_q(p.q + q_at, cs, [&](int i) { return Tile::q_dim(i, g); }, p.rotate, p.scale_log2, x);
         Tile::query(x, q);
     }
     floatx4 o[4] = {};
@@ -1000,8 +1012,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     {
         const float* const cs = reinterpret_cast<const float*>(p.rope + (long long)qpos * kPairs);
         floatx4 x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = scaled_q4(p.q + q_at, cs, 16 * (i >> 1) + 8 * half + 4 * (i & 1), p.rotate, p.scale_log2);
+        load_q(p.q + q_at, cs, [&](int i) { return 16 * (i >> 1) + 8 * half + 4 * (i & 1); }, p.rotate, p.scale_log2, x);
         float up = 1.f;
         if constexpr (P::kScaled) {
             float top = 0.f;
