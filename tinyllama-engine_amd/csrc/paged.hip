@@ -892,10 +892,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     const int n_rows = n_tok * p.gqa, n_rt = (n_rows + kChunkRows - 1) / kChunkRows;
     // Row tiles last first (they see most keys); the items of one tile next to
     // each other, so that with a multiple of 8 of them, or a divisor, the row
-    // tiles that read one range of keys of one head run on the same XCDs.
+    // tiles that read one range of keys of one head run on the same XCDs.  Where
+    // the tiles of a prompt see very different numbers of keys, those XCDs would
+    // have very different numbers of items with any work (a 2048-token prompt in
+    // two parts 66 us): there each row tile starts one place further.
     const int local = item - b.first[rank];
     const int n_combo = (b.first[rank + 1] - b.first[rank]) / n_rt;
-    const int rt = n_rt - 1 - local / n_combo, combo = local % n_combo;
+    const int rt_rank = local / n_combo, rt = n_rt - 1 - rt_rank;
+    const int combo = (local - rt_rank * n_combo + (pos < 4 * n_tok ? rt_rank : 0)) % n_combo;
     const int kvh = combo % p.n_head_kv, split = combo / p.n_head_kv;
     const int row0 = rt * kChunkRows, last_row = min(row0 + kChunkRows, n_rows) - 1;
     const int last_key = pos + last_row / p.gqa;

@@ -65,17 +65,22 @@ inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, P
     b.first[n_seq] = p->n_items = static_cast<int>(at);
 }
 
-// Parts of the keys by estimated time, in tile steps: one round of workgroups
-// takes the longest part, several their even share and half a part for the
-// uneven end; a part costs about three steps of its own (its queries, its first
-// tile, handing over its state).
+// Parts of the keys by estimated time in us, fitted to chunks of 32 to 2048 tokens
+// over 0 to 8000 positions, 32 / 4 heads: a CU takes 0.69 / 0.93 / 1.02 64-key tiles
+// of F16 a us with one, two and three workgroups (4/3 of the time for one of BF16
+// or 32 keys of F32), the longest part alone 1.45 us for each of its tiles; half of
+// the longest part for the uneven end of several rounds; 8 us for a workgroup's
+// start and end, and for handing over 2 us and 1 us a part.  (F16, 512 tokens after
+// 8000 in 1 / 2 / 4 / 6 / 12 parts 190 / 106 / 84.7 / 82.6 / 95 us, estimated 195 / 106 /
+// 88 / 81 / 91; 128 after 8000 in 4 / 8 / 24 54.6 / 36.3 / 46.4; 2048 after 2000 in 1 / 2
+// 117 / 126.)
 inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* p)
 {
     PagedBatch& b = p->batch;
     const int keys = chunk_tile(type);
-    const double slots = 3.0 * n_cu;
+    const double unit = type == kKvF16 ? 1.0 : 4.0 / 3;
     int last[kMaxSeqPerLaunch], most = 0;  // tiles of a sequence's last row tile
-    long long units[kMaxSeqPerLaunch], all = 0;
+    long long units[kMaxSeqPerLaunch];
     double total = 0;
     const auto first_of = [&](int s) { return b.pos[s] / keys + 1; };
     for (int s = 0; s < n_seq; ++s) {
@@ -83,7 +88,6 @@ inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, Pa
         const long long rows = static_cast<long long>(n_tok) * gqa;
         last[s] = rows > kStreamRows ? (b.pos[s] + n_tok - 1) / keys + 1 : 0;
         units[s] = last[s] ? (rows + kChunkRows - 1) / kChunkRows * n_head_kv : 0;
-        all += units[s];
         total += 0.5 * units[s] * (first_of(s) + last[s]);
         most = std::max(most, last[s]);
     }
@@ -92,19 +96,25 @@ inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, Pa
     p->shared = false;
     if (!most) return;
     double best = 0;
+    int worse = 0;
     for (const int parts : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64}) {
         const int len = (most + parts - 1) / parts;
-        if (parts > 1 && (len < 4 || all > 4 * slots)) break;
-        double items = 0;
+        if (parts > 1 && (len < 2 || worse > 3)) break;
+        double items = 0;  // with any work
         for (int s = 0; s < n_seq; ++s) {
             const int lo = (first_of(s) + len - 1) / len, hi = (last[s] + len - 1) / len;
             items += units[s] * (lo == hi ? hi : std::max(1.0, 0.5 * (first_of(s) + last[s]) / len + 0.5));
         }
-        const double steps = (items <= slots ? len : std::max<double>(len, total / slots + 0.5 * len)) +
-                             3 * std::max(1.0, items / slots) + (parts > 1 ? 0.3 * parts : 0);
-        if (parts == 1 || steps < best) {
-            best = steps;
+        const double per_cu = items / n_cu;
+        const double rate = per_cu <= 1 ? 0.69 * per_cu : per_cu <= 2 ? 0.69 + 0.24 * (per_cu - 1) : std::min(1.02, 0.93 + 0.09 * (per_cu - 2));
+        const double us = unit * (std::max(total / (n_cu * rate), 1.45 * len) + (per_cu > 3 ? 0.5 * len : 0)) +
+                          (parts > 1 ? 2.0 + parts : 0);
+        if (parts == 1 || us < best) {
+            best = us;
             p->split_tiles = len;
+            worse = 0;
+        } else {
+            ++worse;
         }
     }
     long long at = 0;
