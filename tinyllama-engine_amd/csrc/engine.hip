@@ -1397,9 +1397,9 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
                         const int* n_tok_host, int layer, int flags, float* out_dev, const float* q_dev)
 {
     PagedAttentionParams p{};
-    PagedPlan plan{};
+    PagedBatch batch{};
     int total = 0;
-    if (int rc = check_paged(e, cache, n_seq, pos_host, n_tok_host, layer, flags, &p.pool, &plan.batch, &total))
+    if (int rc = check_paged(e, cache, n_seq, pos_host, n_tok_host, layer, flags, &p.pool, &batch, &total))
         return rc;
     if (!out_dev || !q_dev) return fail(TLA_ERR_INVALID_ARGUMENT, "NULL device pointer");
     if (!aligned16(out_dev) || !aligned16(q_dev))
@@ -1415,26 +1415,33 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
     p.gqa = e->gqa;
     p.rotate = (flags & TLA_ROTATE) ? 1 : 0;
     p.scale_log2 = scale_log2(e->head_dim);
-    for (const bool chunk : {true, false}) {
-        if (chunk)
-            plan_chunk(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &plan);
-        else
-            plan_stream(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &plan);
-        if (plan.n_items == 0) continue;
-        if (plan.shared) {
-            const size_t items = static_cast<size_t>(plan.n_items);
-            if (int rc = ensure_ws(e, items * (chunk ? kChunkStateBytes : kStreamStateBytes))) return rc;
-            if (int rc = ensure_counters(e, &e->counters, e->n_counters, items * kCounterStride)) return rc;
-            p.part = static_cast<float*>(e->ws);
-            p.counters = e->counters;
-        }
-        p.n_items = plan.n_items;
-        p.split_tiles = plan.split_tiles;
-        if (int rc = launch(e, chunk ? TLA_KERNEL_PREFILL : TLA_KERNEL_DECODE, "paged attention", [&] {
-                return chunk ? launch_paged_chunk(p, plan.batch, e->stream) : launch_paged_stream(p, plan.batch, e->stream);
-            }))
-            return rc;
+    PagedPlan chunks{}, streams{};
+    chunks.batch = streams.batch = batch;
+    plan_chunk(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &chunks);
+    plan_stream(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &streams);
+    p.chunk.n_items = chunks.n_items;
+    p.chunk.split_tiles = chunks.split_tiles;
+    p.stream.n_items = streams.n_items;
+    // The kinds' states and counters side by side (either may run beside the other).
+    const size_t c_items = chunks.shared ? chunks.n_items : 0, s_items = streams.shared ? streams.n_items : 0;
+    if (c_items + s_items) {
+        if (int rc = ensure_ws(e, c_items * kChunkStateBytes + s_items * kStreamStateBytes)) return rc;
+        if (int rc = ensure_counters(e, &e->counters, e->n_counters, (c_items + s_items) * kCounterStride)) return rc;
+        p.chunk.part = static_cast<float*>(e->ws);
+        p.chunk.counters = e->counters;
+        p.stream.part = p.chunk.part + c_items * (kChunkStateBytes / 4);
+        p.stream.counters = e->counters + c_items * kCounterStride;
     }
+    if (p.chunk.n_items && p.stream.n_items && n_seq <= kMaxMixedSeqs && cache->page_size >= 16)
+        return launch(e, TLA_KERNEL_PREFILL, "paged attention",
+                      [&] { return launch_paged_mixed(p, chunks.batch, streams.batch, e->stream); });
+    if (p.chunk.n_items)
+        if (int rc = launch(e, TLA_KERNEL_PREFILL, "paged attention",
+                            [&] { return launch_paged_chunk(p, chunks.batch, e->stream); }))
+            return rc;
+    if (p.stream.n_items)
+        return launch(e, TLA_KERNEL_DECODE, "paged attention",
+                      [&] { return launch_paged_stream(p, streams.batch, e->stream); });
     return ok();
 }
 

@@ -62,19 +62,26 @@ hipError_t launch_paged_append(const PagedAppendParams& p, const PagedBatch& b, 
 // counters of 1024 work items kept a launch of 8 x 16384 positions to 110 us.
 constexpr int kCounterStride = 64;
 
+// The work items of one kind of a call, and the workspace of its own that they
+// share rows through.
+struct PagedWork {
+    float* part;     // softmax states of the items that share rows, by item
+    int* counters;   // and their arrivals, by the rows' first item, kCounterStride apart; zero
+                     // between launches
+    int n_items;     // 0: none of the kind in the call
+    int split_tiles; // chunks: key tiles per item at most
+};
+
 struct PagedAttentionParams {
     PagedPool pool;
     const float* q;  // [total tokens][n_head][64]
     float* out;
     const float2* rope;
-    float* part;     // softmax states of workgroups that share rows, by work item
-    int* counters;   // and their arrivals, by the rows' first work item, kCounterStride apart; zero between launches
+    PagedWork chunk, stream;
     int n_seq;
     int n_head;
     int n_head_kv;
     int gqa;
-    int n_items;
-    int split_tiles; // key tiles per work item at most
     int rotate;
     float scale_log2;
 };
@@ -100,6 +107,10 @@ constexpr int kChunkStateBytes = 4 * 64 * 34 * 4;
 constexpr int chunk_tile(int type) { return type == kKvF32 ? 32 : 64; }
 hipError_t launch_paged_stream(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s);
 hipError_t launch_paged_chunk(const PagedAttentionParams& p, const PagedBatch& b, hipStream_t s);
+// Both kinds at once: pages of at least 16 positions, and no more sequences than
+// two kinds' argument blocks hold in 4 KiB.
+constexpr int kMaxMixedSeqs = 64;
+hipError_t launch_paged_mixed(const PagedAttentionParams& p, const PagedBatch& chunks, const PagedBatch& streams, hipStream_t s);
 
 hipError_t load_paged_code();
 

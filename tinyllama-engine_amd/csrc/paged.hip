@@ -462,16 +462,22 @@ struct StreamTile<kKvF32> {
 // waves of the SIMD cover the wait.
 // kSmall: pages of fewer than 16 positions, whose rows are looked up one by
 // one; else each half of a tile lies in one page, looked up by the wave.
+struct StreamShared {
+    floatx4 o[4][4][kWave];  // [wave][r][lane]
+    float2 ml[4][kWave];
+    int bad[16];
+    int last;
+};
 template <int kType, bool kSmall, int kMaxSeq>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void paged_stream_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
+__device__ __forceinline__ void stream_item(const PagedAttentionParams& p, const PagedWork& work, const PagedSeqs<kMaxSeq>& b,
+                                            const int item, StreamShared& sh)
 {
     typedef typename Elem<kType>::T T;
     typedef StreamTile<kType> Tile;
-    __shared__ floatx4 s_o[4][4][kWave];  // [wave][r][lane]
-    __shared__ float2 s_ml[4][kWave];
-    __shared__ int s_bad[16];
-    __shared__ int s_last;
-    const int item = blockIdx.x;
+    auto& s_o = sh.o;
+    auto& s_ml = sh.ml;
+    auto& s_bad = sh.bad;
+    auto& s_last = sh.last;
     const int rank = rank_of(b, p.n_seq, item), seq = b.id(rank);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kWave - 1);
     const int local = item - b.first[rank];
@@ -645,7 +651,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
         // real rows' are made, and each max and sum is read by one lane, into the
         // LDS that the waves' states leave.
         const unsigned stride = p.n_head_kv * kStreamStateBytes;  // from part to part
-        const auto rs = __builtin_amdgcn_make_buffer_rsrc(p.part + (long long)(b.first[rank] + kvh) * (kStreamStateBytes / 4), 0,
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc(work.part + (long long)(b.first[rank] + kvh) * (kStreamStateBytes / 4), 0,
                                                           n_split * stride, kRawBufferWord3);
         const unsigned o_at = 1024 * wave + 16 * lane, ml_at = 4096;
         if (real) {
@@ -654,7 +660,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
                 __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uintx2, make_float2(m_run, l_run)), rs, ml_at + 8 * c,
                                                       split * stride, kDeviceScope);
         }
-        if (!last_to_arrive(p.counters + (long long)(b.first[rank] + kvh) * kCounterStride, n_split, s_last)) return;
+        if (!last_to_arrive(work.counters + (long long)(b.first[rank] + kvh) * kCounterStride, n_split, s_last)) return;
         float2* const s_part = reinterpret_cast<float2*>(s_o);  // [n_split][16]
         static_assert(sizeof(s_o) >= kMaxStreamParts * 16 * sizeof(float2), "the parts' max and sum");
         for (int i = threadIdx.x; i < 16 * n_split; i += 256)
@@ -875,18 +881,24 @@ struct ChunkTile<kKvF32> {
 // pages) or in registers.
 // kSmall: pages of fewer than 8 positions, whose rows are looked up by each
 // lane; else the eight rows that a wave loads lie in one page.
+template <int kType>
+struct ChunkShared {
+    alignas(16) unsigned char kv[2][ChunkTile<kType>::kSub][ChunkTile<kType>::kBytes];
+    unsigned there[2][ChunkTile<kType>::kSub];  // bit i: key i of the 32 is there
+    int last;
+};
 template <int kType, bool kSmall, int kMaxSeq>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void paged_chunk_kernel(const PagedAttentionParams p, const PagedSeqs<kMaxSeq> b)
+__device__ __forceinline__ void chunk_item(const PagedAttentionParams& p, const PagedWork& work, const PagedSeqs<kMaxSeq>& b,
+                                           const int item, ChunkShared<kType>& sh)
 {
     typedef typename Elem<kType>::T T;
     typedef ChunkTile<kType> Tile;
     typedef Pieces<kType> P;
     typedef typename P::Frag Frag;
     constexpr int kKeys = Tile::kKeys, kSub = Tile::kSub;
-    __shared__ __align__(16) unsigned char s_kv[2][kSub][Tile::kBytes];
-    __shared__ unsigned s_there[2][kSub];  // bit i: key i of the plane is there
-    __shared__ int s_last;
-    const int item = blockIdx.x;
+    auto& s_kv = sh.kv;
+    auto& s_there = sh.there;
+    auto& s_last = sh.last;
     const int rank = rank_of(b, p.n_seq, item), seq = b.id(rank);
     const int pos = b.pos[seq], n_tok = b.tok[seq + 1] - b.tok[seq], len = pos + n_tok;
     const int n_rows = n_tok * p.gqa, n_rt = (n_rows + kChunkRows - 1) / kChunkRows;
@@ -904,9 +916,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     const int row0 = rt * kChunkRows, last_row = min(row0 + kChunkRows, n_rows) - 1;
     const int last_key = pos + last_row / p.gqa;
     const int n_tiles = last_key / kKeys + 1;
-    const int n_split = (n_tiles + p.split_tiles - 1) / p.split_tiles;
+    const int n_split = (n_tiles + work.split_tiles - 1) / work.split_tiles;
     if (split >= n_split) return;  // the whole workgroup
-    const int tile0 = split * p.split_tiles, tile_end = min(tile0 + p.split_tiles, n_tiles);
+    const int tile0 = split * work.split_tiles, tile_end = min(tile0 + work.split_tiles, n_tiles);
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kWave - 1);
     const int col = lane & 31, half = lane >> 5;
@@ -1116,7 +1128,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     if (n_split > 1) {
         const auto part_of = [&](int s) {
             const long long i = b.first[rank] + (long long)(n_rt - 1 - rt) * n_combo + s * p.n_head_kv + kvh;
-            return __builtin_amdgcn_make_buffer_rsrc(p.part + i * (kChunkStateBytes / 4) + wave * (64 * 34), 0, 64 * 34 * 4, kRawBufferWord3);
+            return __builtin_amdgcn_make_buffer_rsrc(work.part + i * (kChunkStateBytes / 4) + wave * (64 * 34), 0, 64 * 34 * 4, kRawBufferWord3);
         };
         const auto mine = part_of(split);
 #pragma unroll
@@ -1127,7 +1139,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, x), mine, 1024 * i + 16 * lane, 0, kDeviceScope);
         }
         __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uintx2, make_float2(m_run, l_run)), mine, 8192 + 8 * lane, 0, kDeviceScope);
-        if (!last_to_arrive(p.counters + (long long)(b.first[rank] + (n_rt - 1 - rt) * n_combo + kvh) * kCounterStride, n_split, s_last)) return;
+        if (!last_to_arrive(work.counters + (long long)(b.first[rank] + (n_rt - 1 - rt) * n_combo + kvh) * kCounterStride, n_split, s_last)) return;
         m_run = -INFINITY;
         l_run = 0.f;
         o[0] = o[1] = floatx16{};
@@ -1184,6 +1196,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
         const float x = q_lane(p.q + at, p.rope + (long long)(pos + ti) * kPairs, p.rotate, p.scale_log2);
         p.out[at + lane] = plain_row<kType>(p.pool, table, kv_dim, head_off, pos + ti, x);
     }
+}
+
+template <int kType, bool kSmall, int kMaxSeq>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void paged_stream_kernel(const PagedAttentionParams p,
+                                                                                                     const PagedSeqs<kMaxSeq> b)
+{
+    __shared__ StreamShared sh;
+    stream_item<kType, kSmall>(p, p.stream, b, blockIdx.x, sh);
+}
+
+template <int kType, bool kSmall, int kMaxSeq>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void paged_chunk_kernel(const PagedAttentionParams p,
+                                                                                                    const PagedSeqs<kMaxSeq> b)
+{
+    __shared__ ChunkShared<kType> sh;
+    chunk_item<kType, kSmall>(p, p.chunk, b, blockIdx.x, sh);
+}
+
+// Chunks and single tokens in one launch, the chunks' items first: either kind
+// alone seldom fills the GPU to its end.
+template <int kType, int kMaxSeq>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void paged_mixed_kernel(
+    const PagedAttentionParams p, const PagedSeqs<kMaxSeq> chunks, const PagedSeqs<kMaxSeq> streams)
+{
+    __shared__ union {
+        ChunkShared<kType> c;
+        StreamShared s;
+    } sh;
+    const int item = blockIdx.x;
+    if (item < p.chunk.n_items)
+        chunk_item<kType, false>(p, p.chunk, chunks, item, sh.c);
+    else
+        stream_item<kType, false>(p, p.stream, streams, item - p.chunk.n_items, sh.s);
 }
 
 // f(batch) with the kernel argument block of the smallest size that holds n
@@ -1246,10 +1291,11 @@ hipError_t launch_paged_stream(const PagedAttentionParams& p, const PagedBatch& 
     return with_type(p.pool.type, [&](auto type) {
         return with_batch(b, p.n_seq, [&](const auto& seqs) {
             constexpr int kMax = sizeof(seqs.pos) / sizeof(int);
+            const dim3 grid(p.stream.n_items);
             if (p.pool.page_shift < 4)
-                hipLaunchKernelGGL((paged_stream_kernel<type.value, true, kMax>), dim3(p.n_items), dim3(256), 0, s, p, seqs);
+                hipLaunchKernelGGL((paged_stream_kernel<type.value, true, kMax>), grid, dim3(256), 0, s, p, seqs);
             else
-                hipLaunchKernelGGL((paged_stream_kernel<type.value, false, kMax>), dim3(p.n_items), dim3(256), 0, s, p, seqs);
+                hipLaunchKernelGGL((paged_stream_kernel<type.value, false, kMax>), grid, dim3(256), 0, s, p, seqs);
         });
     });
 }
@@ -1259,11 +1305,27 @@ hipError_t launch_paged_chunk(const PagedAttentionParams& p, const PagedBatch& b
     return with_type(p.pool.type, [&](auto type) {
         return with_batch(b, p.n_seq, [&](const auto& seqs) {
             constexpr int kMax = sizeof(seqs.pos) / sizeof(int);
+            const dim3 grid(p.chunk.n_items);
             if (p.pool.page_shift < 3)
-                hipLaunchKernelGGL((paged_chunk_kernel<type.value, true, kMax>), dim3(p.n_items), dim3(256), 0, s, p, seqs);
+                hipLaunchKernelGGL((paged_chunk_kernel<type.value, true, kMax>), grid, dim3(256), 0, s, p, seqs);
             else
-                hipLaunchKernelGGL((paged_chunk_kernel<type.value, false, kMax>), dim3(p.n_items), dim3(256), 0, s, p, seqs);
+                hipLaunchKernelGGL((paged_chunk_kernel<type.value, false, kMax>), grid, dim3(256), 0, s, p, seqs);
         });
+    });
+}
+
+hipError_t launch_paged_mixed(const PagedAttentionParams& p, const PagedBatch& chunks, const PagedBatch& streams, hipStream_t s)
+{
+    if (p.pool.page_shift < 4 || p.n_seq > kMaxMixedSeqs) return hipErrorInvalidValue;
+    const dim3 grid(p.chunk.n_items + p.stream.n_items);
+    return with_type(p.pool.type, [&](auto type) {
+        if (p.n_seq <= 8)
+            hipLaunchKernelGGL((paged_mixed_kernel<type.value, 8>), grid, dim3(256), 0, s, p, fewer<8>(chunks, p.n_seq),
+                               fewer<8>(streams, p.n_seq));
+        else
+            hipLaunchKernelGGL((paged_mixed_kernel<type.value, kMaxMixedSeqs>), grid, dim3(256), 0, s, p,
+                               fewer<kMaxMixedSeqs>(chunks, p.n_seq), fewer<kMaxMixedSeqs>(streams, p.n_seq));
+        return hipGetLastError();
     });
 }
 
