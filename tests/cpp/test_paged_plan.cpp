@@ -44,10 +44,11 @@ int main()
                 plan_stream(n_seq, hkv, gqa, n_cu, type, plan.get());
             if (plan->n_items == 0) continue;
             CHECK(plan->n_items == b.first[n_seq] && b.first[0] == 0);
-            bool shared = false;
+            int shared = 0;
+            std::vector<int> ids(n_seq, 0);
             for (int r = 0; r < n_seq; ++r) {
                 const int s = b.id(r), items = b.first[r + 1] - b.first[r];
-                CHECK(items >= 0);
+                CHECK(items >= 0 && ++ids[s] == 1);
                 const int n_tok = b.tok[s + 1] - b.tok[s], len = b.pos[s] + n_tok, rows = n_tok * gqa;
                 if (!items) continue;
                 ++served[s];
@@ -57,7 +58,7 @@ int main()
                     const int n_split = items / hkv, n_tiles = (len + kStreamTile - 1) / kStreamTile;
                     const int per = (n_tiles + n_split - 1) / n_split;
                     CHECK(static_cast<long long>(per) * n_split >= n_tiles);
-                    shared |= n_split > 1;
+                    if (n_split > 1) shared = b.first[r + 1];
                     CHECK(n_split == 1 || per >= 2);
                     CHECK(n_split <= kMaxStreamParts);
                 } else {
@@ -70,11 +71,11 @@ int main()
                         const int n_tiles = (b.pos[s] + last_row / gqa) / keys + 1;
                         const int n_split = (n_tiles + plan->split_tiles - 1) / plan->split_tiles;
                         CHECK(n_split >= 1 && n_split <= splits);
-                        shared |= n_split > 1;
+                        if (n_split > 1) shared = b.first[r + 1];
                     }
                 }
             }
-            CHECK(plan->shared || !shared);
+            CHECK(plan->n_shared >= shared && plan->n_shared <= plan->n_items);
         }
         for (int s = 0; s < n_seq; ++s) CHECK(served[s] == (b.tok[s + 1] > b.tok[s] ? 1 : 0));
     }

@@ -1423,7 +1423,9 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
     p.chunk.split_tiles = chunks.split_tiles;
     p.stream.n_items = streams.n_items;
     // The kinds' states and counters side by side (either may run beside the other).
-    const size_t c_items = chunks.shared ? chunks.n_items : 0, s_items = streams.shared ? streams.n_items : 0;
+    if (chunks.n_items >= kMaxPagedItems || streams.n_items >= kMaxPagedItems)
+        return fail(TLA_ERR_UNSUPPORTED, "%d tokens are more than one call takes", total);
+    const size_t c_items = chunks.n_shared, s_items = streams.n_shared;
     if (c_items + s_items) {
         if (int rc = ensure_ws(e, c_items * kChunkStateBytes + s_items * kStreamStateBytes)) return rc;
         if (int rc = ensure_counters(e, &e->counters, e->n_counters, (c_items + s_items) * kCounterStride)) return rc;

@@ -98,8 +98,9 @@ struct PagedPlan {
     PagedBatch batch;  // pos and tok set by the caller
     int n_items;       // 0: no such sequence in the call
     int split_tiles;
-    bool shared;       // some rows are shared by several work items
+    int n_shared;      // the items before this one may share rows with others
 };
+constexpr int kMaxPagedItems = 1 << 30;  // n_items of a plan that has more than a launch takes
 // Bytes of one work item's softmax state.
 constexpr int kStreamStateBytes = 64 * 18 * 4;
 constexpr int kChunkStateBytes = 4 * 64 * 34 * 4;

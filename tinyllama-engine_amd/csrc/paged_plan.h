@@ -7,6 +7,29 @@
 
 namespace tla {
 
+// Hands out the work items, tiles[s] key tiles in parts of at most p->split_tiles
+// times units(s) for sequence s: the longest sequences first, so that the last
+// items to start are short ones and those that share rows come before all others.
+template <class F>
+inline void rank_items(int n_seq, const int* tiles, F&& units, PagedPlan* p)
+{
+    PagedBatch& b = p->batch;
+    long long order[kMaxSeqPerLaunch];  // descending tiles, then ascending sequence
+    for (int s = 0; s < n_seq; ++s) order[s] = -(static_cast<long long>(tiles[s]) << 8) + s;
+    if (!std::is_sorted(order, order + n_seq)) std::sort(order, order + n_seq);
+    long long at = 0;
+    p->n_shared = 0;
+    for (int r = 0; r < n_seq; ++r) {
+        const int s = static_cast<int>(order[r] & 255);
+        b.first[r] = static_cast<int>(std::min<long long>(at, kMaxPagedItems));
+        b.set_id(r, s);
+        const int n = (tiles[s] + p->split_tiles - 1) / p->split_tiles;
+        at += n * static_cast<long long>(units(s));
+        if (n > 1) p->n_shared = static_cast<int>(std::min<long long>(at, kMaxPagedItems));
+    }
+    b.first[n_seq] = p->n_items = static_cast<int>(std::min<long long>(at, kMaxPagedItems));
+}
+
 // Parts of the keys by estimated time in us, fitted to launches of 1 to 200
 // sequences of 128 to 16384 positions, 32 / 4 heads (F16, one sequence of 16384
 // positions in 16 / 32 / 64 / 128 parts 15.5 / 14.1 / 17.1 / 26.6 us; 64 of 1100
@@ -29,8 +52,7 @@ inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, P
         most = std::max(most, tiles[s]);
         total += tiles[s];
     }
-    p->n_items = 0;
-    p->shared = false;
+    p->n_items = p->n_shared = 0;
     if (!most) return;
     p->split_tiles = most;
     double best = 0;
@@ -54,15 +76,7 @@ inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, P
             ++worse;
         }
     }
-    long long at = 0;
-    for (int s = 0; s < n_seq; ++s) {
-        b.first[s] = static_cast<int>(at);
-        b.set_id(s, s);
-        const int n = (tiles[s] + p->split_tiles - 1) / p->split_tiles;
-        p->shared |= n > 1;
-        at += static_cast<long long>(n) * n_head_kv;
-    }
-    b.first[n_seq] = p->n_items = static_cast<int>(at);
+    rank_items(n_seq, tiles, [&](int) { return n_head_kv; }, p);
 }
 
 // Parts of the keys by estimated time in us, fitted to chunks of 32 to 2048 tokens
@@ -92,8 +106,7 @@ inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, Pa
         most = std::max(most, last[s]);
     }
     p->split_tiles = std::max(most, 1);
-    p->n_items = 0;
-    p->shared = false;
+    p->n_items = p->n_shared = 0;
     if (!most) return;
     double best = 0;
     int worse = 0;
@@ -117,15 +130,7 @@ inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, Pa
             ++worse;
         }
     }
-    long long at = 0;
-    for (int s = 0; s < n_seq; ++s) {
-        b.first[s] = static_cast<int>(at);
-        b.set_id(s, s);
-        const int n = (last[s] + p->split_tiles - 1) / p->split_tiles;
-        p->shared |= n > 1;
-        at += n * units[s];
-    }
-    b.first[n_seq] = p->n_items = static_cast<int>(at);
+    rank_items(n_seq, last, [&](int s) { return units[s]; }, p);
 }
 
 }  // namespace tla
