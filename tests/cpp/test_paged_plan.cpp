@@ -37,11 +37,10 @@ int main()
         }
         b.tok[n_seq] = t;
         std::vector<int> served(n_seq, 0);
+        auto streams = std::make_unique<PagedPlan>();
+        plan_attention(n_seq, hkv, gqa, n_cu, type, plan.get(), streams.get());
         for (const bool chunk : {true, false}) {
-            if (chunk)
-                plan_chunk(n_seq, hkv, gqa, n_cu, type, plan.get());
-            else
-                plan_stream(n_seq, hkv, gqa, n_cu, type, plan.get());
+            if (!chunk) std::swap(*plan, *streams);
             if (plan->n_items == 0) continue;
             CHECK(plan->n_items == b.first[n_seq] && b.first[0] == 0);
             int shared = 0;
@@ -54,10 +53,15 @@ int main()
                 ++served[s];
                 CHECK(items % hkv == 0);
                 if (!chunk) {
-                    CHECK(rows >= 1 && rows <= kStreamRows);
-                    const int n_split = items / hkv, n_tiles = (len + kStreamTile - 1) / kStreamTile;
+                    const int n_unit = stream_units(rows, hkv);
+                    CHECK(items % n_unit == 0);
+                    CHECK(rows >= 1 && rows <= kStreamRowsMost);
+                    const int n_split = items / n_unit, n_tiles = (len + kStreamTile - 1) / kStreamTile;
+                    for (int row0 = 0; row0 < rows; row0 += 16) {  // each unit's tiles in equal parts
+                        const int n = (b.pos[s] + (std::min(row0 + 16, rows) - 1) / gqa) / kStreamTile + 1;
+                        CHECK(n >= 1 && n <= n_tiles && static_cast<long long>((n + n_split - 1) / n_split) * n_split >= n);
+                    }
                     const int per = (n_tiles + n_split - 1) / n_split;
-                    CHECK(static_cast<long long>(per) * n_split >= n_tiles);
                     if (n_split > 1) shared = b.first[r + 1];
                     CHECK(n_split == 1 || per >= 2);
                     CHECK(n_split <= kMaxStreamParts);

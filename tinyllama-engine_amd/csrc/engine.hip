@@ -1397,9 +1397,9 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
                         const int* n_tok_host, int layer, int flags, float* out_dev, const float* q_dev)
 {
     PagedAttentionParams p{};
-    PagedBatch batch{};
+    PagedPlan chunks{}, streams{};
     int total = 0;
-    if (int rc = check_paged(e, cache, n_seq, pos_host, n_tok_host, layer, flags, &p.pool, &batch, &total))
+    if (int rc = check_paged(e, cache, n_seq, pos_host, n_tok_host, layer, flags, &p.pool, &chunks.batch, &total))
         return rc;
     if (!out_dev || !q_dev) return fail(TLA_ERR_INVALID_ARGUMENT, "NULL device pointer");
     if (!aligned16(out_dev) || !aligned16(q_dev))
@@ -1415,10 +1415,7 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
     p.gqa = e->gqa;
     p.rotate = (flags & TLA_ROTATE) ? 1 : 0;
     p.scale_log2 = scale_log2(e->head_dim);
-    PagedPlan chunks{}, streams{};
-    chunks.batch = streams.batch = batch;
-    plan_chunk(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &chunks);
-    plan_stream(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &streams);
+    plan_attention(n_seq, p.n_head_kv, p.gqa, e->n_cu, p.pool.type, &chunks, &streams);
     p.chunk.n_items = chunks.n_items;
     p.chunk.split_tiles = chunks.split_tiles;
     p.stream.n_items = streams.n_items;

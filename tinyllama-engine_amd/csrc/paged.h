@@ -86,11 +86,19 @@ struct PagedAttentionParams {
     float scale_log2;
 };
 
-// How one call's sequences are served: those of at most kStreamRows query rows
-// per kv head stream their keys and values past rows held in registers
-// (paged_stream_kernel), longer chunks go through LDS tiles
-// (paged_chunk_kernel).
-constexpr int kStreamRows = 16;
+// How one call's sequences are served: those of at most `rows` query rows per kv
+// head stream their keys and values past 16 rows held in registers
+// (paged_stream_kernel; further rows read them again, from the L2), longer chunks
+// go through LDS tiles (paged_chunk_kernel), which need a third of the time for each
+// product but more before the first and after the last.  Up to kStreamRows rows
+// streaming was faster throughout (F16, 4 kv heads, 64 rows over 500 / 4000 / 16000
+// positions 7.3 / 9.5 / 15.6 us against 11.9 / 22.3 / 37.9; 16 sequences of 1500 16.9
+// against 20.2); up to kStreamRowsMost the plans' estimates decide (128 rows: 8.0 /
+// 10.2 / 22.0 against 13.3 / 22.9 / 38.6; 16 of 1500 23.7 against 21.9).
+constexpr int kStreamRows = 64;
+constexpr int kStreamRowsMost = 2048;
+// Units of 16 rows of one kv head that a streamed sequence of `rows` rows has.
+__host__ __device__ constexpr int stream_units(int rows, int n_head_kv) { return (rows + 15) / 16 * n_head_kv; }
 constexpr int kStreamTile = 32;  // keys per tile of one wave
 constexpr int kMaxStreamParts = 128;  // work items that share a row
 constexpr int kChunkRows = 128;  // query rows of a workgroup
@@ -98,6 +106,7 @@ struct PagedPlan {
     PagedBatch batch;  // pos and tok set by the caller
     int n_items;       // 0: no such sequence in the call
     int split_tiles;
+    double us;         // its estimated time
     int n_shared;      // the items before this one may share rows with others
 };
 constexpr int kMaxPagedItems = 1 << 30;  // n_items of a plan that has more than a launch takes

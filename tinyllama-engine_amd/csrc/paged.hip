@@ -452,8 +452,8 @@ struct StreamTile<kKvF32> {
     }
 };
 
-// Rows of one sequence and kv head: up to 16 (token, head) pairs, row c being
-// token c / gqa, head c % gqa of the kv head.  One work item is an equal part of
+// Rows of one sequence and kv head: 16 (token, head) pairs, row i being token
+// i / gqa, head i % gqa of the kv head.  One work item is an equal part of
 // the unit's 32-key tiles, its four waves taking every fourth tile each, with
 // no word to each other until the end: then the waves' states meet in LDS,
 // and the items of one unit in the workspace, where the last to arrive adds
@@ -480,18 +480,17 @@ __device__ __forceinline__ void stream_item(const PagedAttentionParams& p, const
     auto& s_last = sh.last;
     const int rank = rank_of(b, p.n_seq, item), seq = b.id(rank);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kWave - 1);
-    const int local = item - b.first[rank];
-    const int kvh = local % p.n_head_kv, split = local / p.n_head_kv;
-    const int n_split = (b.first[rank + 1] - b.first[rank]) / p.n_head_kv;
-    const int pos = b.pos[seq], n_tok = b.tok[seq + 1] - b.tok[seq];
-    const int len = pos + n_tok, n_rows = n_tok * p.gqa;
-    const int n_tiles = (len + kStreamTile - 1) / kStreamTile;
+    const int pos = b.pos[seq], n_tok = b.tok[seq + 1] - b.tok[seq], len = pos + n_tok;
+    const int n_unit = stream_units(n_tok * p.gqa, p.n_head_kv), local = item - b.first[rank];
+    const int unit = local % n_unit, split = local / n_unit, n_split = (b.first[rank + 1] - b.first[rank]) / n_unit;
+    const int kvh = unit % p.n_head_kv, row0 = 16 * (unit / p.n_head_kv), n_rows = min(16, n_tok * p.gqa - row0);
+    const int n_tiles = (pos + (row0 + n_rows - 1) / p.gqa) / kStreamTile + 1;  // up to its last row's position
     const int c = lane & 15, g = lane >> 4;
     const int* const table = p.pool.table + (long long)seq * p.pool.table_stride;
     const int kv_dim = p.n_head_kv * kHeadDim, head_off = kvh * kHeadDim;
 
     // The row's query.  Rows past the last repeat it (their results are not stored).
-    const int row = min(c, n_rows - 1), t = row / p.gqa, qpos = pos + t;
+    const int row = row0 + min(c, n_rows - 1), t = row / p.gqa, qpos = pos + t;
     const long long q_at = ((long long)(b.tok[seq] + t) * p.n_head + kvh * p.gqa + row - t * p.gqa) * kHeadDim;
     const float* const cs = reinterpret_cast<const float*>(p.rope + (long long)qpos * kPairs);
     if (threadIdx.x < 16) s_bad[threadIdx.x] = 0;
@@ -591,7 +590,7 @@ __device__ __forceinline__ void stream_item(const PagedAttentionParams& p, const
         for (int hf = 0; hf < 2; ++hf) s[hf] = kv.scores(hf, q);
         if (more) load_k(tile + 4);  // into the registers just read
         const int key = tile * kStreamTile + 4 * g;
-        if (kSmall || (tile + 1) * kStreamTile > pos + 1 || !there.half[0] || !there.half[1]) {
+        if (kSmall || (tile + 1) * kStreamTile > pos + row0 / p.gqa + 1 || !there.half[0] || !there.half[1]) {
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -650,8 +649,8 @@ __device__ __forceinline__ void stream_item(const PagedAttentionParams& p, const
         // Parts in order.  A CU's device-scope loads bring about 14 GB/s here: only
         // real rows' are made, and each max and sum is read by one lane, into the
         // LDS that the waves' states leave.
-        const unsigned stride = p.n_head_kv * kStreamStateBytes;  // from part to part
-        const auto rs = __builtin_amdgcn_make_buffer_rsrc(work.part + (long long)(b.first[rank] + kvh) * (kStreamStateBytes / 4), 0,
+        const unsigned stride = n_unit * kStreamStateBytes;  // from part to part
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc(work.part + (long long)(b.first[rank] + unit) * (kStreamStateBytes / 4), 0,
                                                           n_split * stride, kRawBufferWord3);
         const unsigned o_at = 1024 * wave + 16 * lane, ml_at = 4096;
         if (real) {
@@ -660,7 +659,7 @@ __device__ __forceinline__ void stream_item(const PagedAttentionParams& p, const
                 __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uintx2, make_float2(m_run, l_run)), rs, ml_at + 8 * c,
                                                       split * stride, kDeviceScope);
         }
-        if (!last_to_arrive(work.counters + (long long)(b.first[rank] + kvh) * kCounterStride, n_split, s_last)) return;
+        if (!last_to_arrive(work.counters + (long long)(b.first[rank] + unit) * kCounterStride, n_split, s_last)) return;
         float2* const s_part = reinterpret_cast<float2*>(s_o);  // [n_split][16]
         static_assert(sizeof(s_o) >= kMaxStreamParts * 16 * sizeof(float2), "the parts' max and sum");
         for (int i = threadIdx.x; i < 16 * n_split; i += 256)
@@ -701,8 +700,8 @@ __device__ __forceinline__ void stream_item(const PagedAttentionParams& p, const
     // Rows that met something infinite or NaN, seen or not, once more in plain fp32.
     for (int i = wave; i < n_rows; i += 4) {
         if (!s_bad[i]) continue;
-        const int ti = i / p.gqa;
-        const long long at = ((long long)(b.tok[seq] + ti) * p.n_head + kvh * p.gqa + i - ti * p.gqa) * kHeadDim;
+        const int ti = (row0 + i) / p.gqa;
+        const long long at = ((long long)(b.tok[seq] + ti) * p.n_head + kvh * p.gqa + row0 + i - ti * p.gqa) * kHeadDim;
         const float x = q_lane(p.q + at, p.rope + (long long)(pos + ti) * kPairs, p.rotate, p.scale_log2);
         p.out[at + lane] = plain_row<kType>(p.pool, table, kv_dim, head_off, pos + ti, x);
     }

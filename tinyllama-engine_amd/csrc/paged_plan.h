@@ -40,19 +40,24 @@ inline void rank_items(int n_seq, const int* tiles, F&& units, PagedPlan* p)
 // less the more items a CU has; handing over, and adding one part after the other;
 // each further round of four workgroups per CU (96 of 125 to 1000 in 1080 / 700
 // items 21.1 / 17.2).
-inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* p)
+inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, int rows, PagedPlan* p)
 {
     PagedBatch& b = p->batch;
-    const double memory = (type == kKvF32 ? 2.6e-3 : 1.3e-3) * 256 / n_cu, step = type == kKvF32 ? 0.4 : 0.19;
-    int tiles[kMaxSeqPerLaunch], most = 0;
-    double total = 0;
+    const double memory = (type == kKvF32 ? 2.6e-3 : 1.3e-3) * 256 / n_cu, compute = (type == kKvF32 ? 1.65e-3 : 0.85e-3) * 256 / n_cu;
+    const double step = type == kKvF32 ? 0.4 : 0.19;
+    int tiles[kMaxSeqPerLaunch], units[kMaxSeqPerLaunch], most = 0;
+    double total = 0, distinct = 0;  // tiles of all units, and without those read again
     for (int s = 0; s < n_seq; ++s) {
         const int n_tok = b.tok[s + 1] - b.tok[s];
-        tiles[s] = n_tok > 0 && n_tok * gqa <= kStreamRows ? (b.pos[s] + n_tok + kStreamTile - 1) / kStreamTile : 0;
+        tiles[s] = n_tok > 0 && n_tok <= rows / gqa ? (b.pos[s] + n_tok + kStreamTile - 1) / kStreamTile : 0;
+        units[s] = tiles[s] ? stream_units(n_tok * gqa, n_head_kv) : 0;
         most = std::max(most, tiles[s]);
-        total += tiles[s];
+        // a unit's tiles end with its last row's position
+        total += 0.5 * units[s] * (tiles[s] + b.pos[s] / kStreamTile + (tiles[s] ? 1 : 0));
+        distinct += static_cast<double>(tiles[s]) * n_head_kv;
     }
     p->n_items = p->n_shared = 0;
+    p->us = 0;
     if (!most) return;
     p->split_tiles = most;
     double best = 0;
@@ -62,11 +67,10 @@ inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, P
         const int len = (most + parts - 1) / parts;
         if (parts > 1 && (len < 4 || worse > 3)) break;  // a tile for each wave
         long long items = 0;
-        for (int s = 0; s < n_seq; ++s) items += (tiles[s] + len - 1) / len;
-        items *= n_head_kv;
+        for (int s = 0; s < n_seq; ++s) items += static_cast<long long>((tiles[s] + len - 1) / len) * units[s];
         const double per_item = static_cast<double>(n_cu) / items;  // CUs
-        const double us = std::max(total * n_head_kv * memory * std::max(1.0, per_item), len * step) +
-                          (total * n_head_kv < 0.8 * len * items ? 0.14 * len * std::min(1.0, per_item) : 0) +
+        const double us = std::max(std::max(distinct * memory, total * compute) * std::max(1.0, per_item), len * step) +
+                          (total < 0.8 * len * items ? 0.14 * len * std::min(1.0, per_item) : 0) +
                           (parts > 1 ? 2.2 + 0.15 * parts : 0) + 3.0 * ((items - 1) / (4 * n_cu));
         if (parts == 1 || us < best) {
             best = us;
@@ -76,7 +80,8 @@ inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, P
             ++worse;
         }
     }
-    rank_items(n_seq, tiles, [&](int) { return n_head_kv; }, p);
+    p->us = 3 + best;
+    rank_items(n_seq, tiles, [&](int s) { return units[s]; }, p);
 }
 
 // Parts of the keys by estimated time in us, fitted to chunks of 32 to 2048 tokens
@@ -88,7 +93,7 @@ inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, P
 // 8000 in 1 / 2 / 4 / 6 / 12 parts 190 / 106 / 84.7 / 82.6 / 95 us, estimated 195 / 106 /
 // 88 / 81 / 91; 128 after 8000 in 4 / 8 / 24 54.6 / 36.3 / 46.4; 2048 after 2000 in 1 / 2
 // 117 / 126.)
-inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* p)
+inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, int stream_rows, PagedPlan* p)
 {
     PagedBatch& b = p->batch;
     const int keys = chunk_tile(type);
@@ -100,13 +105,14 @@ inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, Pa
     for (int s = 0; s < n_seq; ++s) {
         const int n_tok = b.tok[s + 1] - b.tok[s];
         const long long rows = static_cast<long long>(n_tok) * gqa;
-        last[s] = rows > kStreamRows ? (b.pos[s] + n_tok - 1) / keys + 1 : 0;
+        last[s] = rows > stream_rows ? (b.pos[s] + n_tok - 1) / keys + 1 : 0;
         units[s] = last[s] ? (rows + kChunkRows - 1) / kChunkRows * n_head_kv : 0;
         total += 0.5 * units[s] * (first_of(s) + last[s]);
         most = std::max(most, last[s]);
     }
     p->split_tiles = std::max(most, 1);
     p->n_items = p->n_shared = 0;
+    p->us = 0;
     if (!most) return;
     double best = 0;
     int worse = 0;
@@ -130,7 +136,25 @@ inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, Pa
             ++worse;
         }
     }
+    p->us = 2 + best;
     rank_items(n_seq, last, [&](int s) { return units[s]; }, p);
+}
+
+// Both kinds of a call's work; positions and tokens set in chunks->batch.
+inline void plan_attention(int n_seq, int n_head_kv, int gqa, int n_cu, int type, PagedPlan* chunks, PagedPlan* streams)
+{
+    streams->batch = chunks->batch;
+    plan_chunk(n_seq, n_head_kv, gqa, n_cu, type, kStreamRows, chunks);
+    plan_stream(n_seq, n_head_kv, gqa, n_cu, type, kStreamRows, streams);
+    if (!chunks->n_items) return;
+    PagedPlan c{}, s{};
+    c.batch = s.batch = chunks->batch;
+    plan_stream(n_seq, n_head_kv, gqa, n_cu, type, kStreamRowsMost, &s);
+    if (s.us >= chunks->us + streams->us) return;
+    plan_chunk(n_seq, n_head_kv, gqa, n_cu, type, kStreamRowsMost, &c);
+    if (c.us + s.us >= chunks->us + streams->us) return;
+    *chunks = c;
+    *streams = s;
 }
 
 }  // namespace tla
