@@ -94,9 +94,10 @@ struct PagedAttentionParams {
 // streaming was faster throughout (F16, 4 kv heads, 64 rows over 500 / 4000 / 16000
 // positions 7.3 / 9.5 / 15.6 us against 11.9 / 22.3 / 37.9; 16 sequences of 1500 16.9
 // against 20.2); up to kStreamRowsMost the plans' estimates decide (128 rows: 8.0 /
-// 10.2 / 22.0 against 13.3 / 22.9 / 38.6; 16 of 1500 23.7 against 21.9).
+// 10.2 / 22.0 against 13.3 / 22.9 / 38.6; 16 of 1500 23.7 against 21.9; a prompt of
+// 512 tokens, 4096 rows, 16.1 either way, over F32 22.1 against 23.5).
 constexpr int kStreamRows = 64;
-constexpr int kStreamRowsMost = 2048;
+constexpr int kStreamRowsMost = 4096;
 // Units of 16 rows of one kv head that a streamed sequence of `rows` rows has.
 __host__ __device__ constexpr int stream_units(int rows, int n_head_kv) { return (rows + 15) / 16 * n_head_kv; }
 constexpr int kStreamTile = 32;  // keys per tile of one wave
