@@ -83,6 +83,32 @@ int main()
         }
         for (int s = 0; s < n_seq; ++s) CHECK(served[s] == (b.tok[s + 1] > b.tok[s] ? 1 : 0));
     }
+    // One sequence of 4096 rows in each of 64 kv heads after millions of positions,
+    // beside short ones: the parts' states stay within the 32 bits that address them
+    // (so many units are more work items than further parts would be worth).
+    for (int n_case = 4000; n_case < 4200; ++n_case) {
+        const int n_seq = pick(1, 64), hkv = 64;
+        auto plan = std::make_unique<PagedPlan>();
+        PagedBatch& b = plan->batch;
+        for (int s = 0; s < n_seq; ++s) {
+            b.pos[s] = s == 0 ? pick(1 << 20, 1 << 27) : pick(0, 1000);
+            b.tok[s + 1] = b.tok[s] + (s == 0 ? 4096 : pick(1, 4096));
+        }
+        plan_stream(n_seq, hkv, 1, 256, kKvF16, kStreamRowsMost, plan.get());
+        for (int r = 0; r < n_seq; ++r) {
+            const int s = b.id(r), n = b.first[r + 1] - b.first[r];
+            const int units = stream_units(b.tok[s + 1] - b.tok[s], hkv);
+            CHECK(n % units == 0 && (n == units || static_cast<long long>(n) * kStreamStateBytes < 1ll << 32));
+        }
+    }
+    // More items than a launch takes are told apart from any that it does.
+    {
+        const int n_case = 5000, n_seq = 256;
+        auto plan = std::make_unique<PagedPlan>();
+        for (int s = 0; s < n_seq; ++s) plan->batch.tok[s + 1] = plan->batch.tok[s] + (1 << 16);
+        plan_chunk(n_seq, 1024, 16, 256, kKvF16, kStreamRows, plan.get());
+        CHECK(plan->n_items == kMaxPagedItems);
+    }
     std::printf("plans hold\n");
     return 0;
 }

@@ -1420,7 +1420,7 @@ int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, 
     p.chunk.split_tiles = chunks.split_tiles;
     p.stream.n_items = streams.n_items;
     // The kinds' states and counters side by side (either may run beside the other).
-    if (chunks.n_items >= kMaxPagedItems || streams.n_items >= kMaxPagedItems)
+    if (chunks.n_items + streams.n_items >= kMaxPagedItems)
         return fail(TLA_ERR_UNSUPPORTED, "%d tokens are more than one call takes", total);
     const size_t c_items = chunks.n_shared, s_items = streams.n_shared;
     if (c_items + s_items) {

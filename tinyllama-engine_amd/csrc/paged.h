@@ -110,7 +110,8 @@ struct PagedPlan {
     double us;         // its estimated time
     int n_shared;      // the items before this one may share rows with others
 };
-constexpr int kMaxPagedItems = 1 << 30;  // n_items of a plan that has more than a launch takes
+constexpr int kMaxPagedItems = (1 << 24) - 1;  // a launch's threads, 256 to an item, are counted in 32 bits; a
+                                               // plan of that many or more says this
 // Bytes of one work item's softmax state.
 constexpr int kStreamStateBytes = 64 * 18 * 4;
 constexpr int kChunkStateBytes = 4 * 64 * 34 * 4;
