@@ -84,20 +84,21 @@ inline void plan_stream(int n_seq, int n_head_kv, int gqa, int n_cu, int type, i
     rank_items(n_seq, tiles, [&](int s) { return units[s]; }, p);
 }
 
-// Parts of the keys by estimated time in us, fitted to chunks of 32 to 2048 tokens
-// over 0 to 8000 positions, 32 / 4 heads: a CU takes 0.69 / 0.93 / 1.02 64-key tiles
-// of F16 a us with one, two and three workgroups (4/3 of the time for one of BF16
-// or 32 keys of F32), the longest part alone 1.45 us for each of its tiles; half of
-// the longest part for the uneven end of several rounds; 8 us for a workgroup's
-// start and end, and for handing over 2 us and 1 us a part.  (F16, 512 tokens after
-// 8000 in 1 / 2 / 4 / 6 / 12 parts 190 / 106 / 84.7 / 82.6 / 95 us, estimated 195 / 106 /
-// 88 / 81 / 91; 128 after 8000 in 4 / 8 / 24 54.6 / 36.3 / 46.4; 2048 after 2000 in 1 / 2
-// 117 / 126.)
+// Parts of the keys by estimated time in us, fitted to 33 calls of 1 to 16 chunks of
+// 128 to 4096 tokens over 0 to 8000 positions, in 1 to 12 parts (to 12%): a CU takes
+// 0.76 / 0.92 / 1.15 64-key tiles of F16 a us with one, two and three workgroups (1.3
+// times the time for one of BF16 or 32 keys of F32), the longest part alone 1.3 us for
+// each of its tiles; a third of the longest part for the uneven end, twice that in
+// several rounds; 8 us for a workgroup's start and end, and for handing over 0.75 us
+// a part and 1.65 us for each work item of a CU.  (F16, 512 tokens after 8000 in 1 /
+// 2 / 4 / 6 / 12 parts 191 / 112 / 87.7 / 85.3 / 98.6 us, 4 x 1500 after none in 1 / 2 / 3 / 6
+// 106 / 104 / 117 / 142; BF16, 8 kv heads, 2 x 900 after 300 in 1 / 2 / 3 / 8 55.7 / 48.8 /
+// 53.3 / 58.2.)
 inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, int stream_rows, PagedPlan* p)
 {
     PagedBatch& b = p->batch;
     const int keys = chunk_tile(type);
-    const double unit = type == kKvF16 ? 1.0 : 4.0 / 3;
+    const double unit = type == kKvF16 ? 1.0 : type == kKvBF16 ? 1.33 : 1.3;
     int last[kMaxSeqPerLaunch], most = 0;  // tiles of a sequence's last row tile
     long long units[kMaxSeqPerLaunch];
     double total = 0;
@@ -125,9 +126,9 @@ inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, in
             items += units[s] * (lo == hi ? hi : std::max(1.0, 0.5 * (first_of(s) + last[s]) / len + 0.5));
         }
         const double per_cu = items / n_cu;
-        const double rate = per_cu <= 1 ? 0.69 * per_cu : per_cu <= 2 ? 0.69 + 0.24 * (per_cu - 1) : std::min(1.02, 0.93 + 0.09 * (per_cu - 2));
-        const double us = unit * (std::max(total / (n_cu * rate), 1.45 * len) + (per_cu > 3 ? 0.5 * len : 0)) +
-                          (parts > 1 ? 2.0 + parts : 0);
+        const double rate = per_cu <= 1 ? 0.76 * per_cu : per_cu <= 2 ? 0.76 + 0.16 * (per_cu - 1) : std::min(1.15, 0.92 + 0.23 * (per_cu - 2));
+        const double us = unit * (std::max(total / (n_cu * rate), 1.3 * len) + (per_cu > 3 ? 0.6 : 0.3) * len) +
+                          (parts > 1 ? 0.5 + 0.75 * std::min(parts, (most + len - 1) / len) + 1.65 * per_cu : 0);
         if (parts == 1 || us < best) {
             best = us;
             p->split_tiles = len;
@@ -136,8 +137,14 @@ inline void plan_chunk(int n_seq, int n_head_kv, int gqa, int n_cu, int type, in
             ++worse;
         }
     }
-    p->us = 2 + best;
+    p->us = 8 + best;
     rank_items(n_seq, last, [&](int s) { return units[s]; }, p);
+}
+
+// Both kinds in one launch start and end side by side.
+inline double launch_us(const PagedPlan& chunks, const PagedPlan& streams)
+{
+    return chunks.us + streams.us - (chunks.n_items && streams.n_items ? 8 : 0);
 }
 
 // Both kinds of a call's work; positions and tokens set in chunks->batch.
@@ -150,9 +157,10 @@ inline void plan_attention(int n_seq, int n_head_kv, int gqa, int n_cu, int type
     PagedPlan c{}, s{};
     c.batch = s.batch = chunks->batch;
     plan_stream(n_seq, n_head_kv, gqa, n_cu, type, kStreamRowsMost, &s);
-    if (s.us >= chunks->us + streams->us) return;
+    const double us = launch_us(*chunks, *streams);
+    if (s.us >= us) return;
     plan_chunk(n_seq, n_head_kv, gqa, n_cu, type, kStreamRowsMost, &c);
-    if (c.us + s.us >= chunks->us + streams->us) return;
+    if (launch_us(c, s) >= us) return;
     *chunks = c;
     *streams = s;
 }
