@@ -443,7 +443,11 @@ int tla_paged_append(tla_engine* e, const tla_paged_cache* cache, int n_seq, con
  * single tokens and chunks of prompts.  q_dev, out_dev [total tokens][n_head]
  * [64] fp32, 16-byte aligned (they may be the same); TLA_ROTATE rotates q.
  * fp32 accuracy for every element type; keys and values that are seen and
- * not finite give what fp32 gives.  Limits as tla_paged_append's. */
+ * not finite give what fp32 gives.  Limits as tla_paged_append's.  Engine memory it
+ * keeps for later calls: softmax states of rows whose keys several workgroups share
+ * (4.5 KiB for 16 streamed rows, 34 KiB for 128 rows of a chunk, for each part of the
+ * keys) and their arrival counters, grown (after a stream synchronize) when a call
+ * needs more. */
 int tla_paged_attention(tla_engine* e, const tla_paged_cache* cache, int n_seq, const int* pos_host,
                         const int* n_tok_host, int layer, int flags, float* out_dev, const float* q_dev);
 
@@ -475,7 +479,9 @@ typedef struct tla_logit_rules {
  * (which may be the same) and, unless tokens_dev is NULL, writes each row's
  * first index of the largest result to tokens_dev [n_seq]: -1 where nothing
  * above -inf is left; a NaN never wins.  Each operation is rounded to fp32 on
- * its own.  Up to 65536 rows, n_vocab up to 2^28. */
+ * its own.  Up to 65536 rows, n_vocab up to 2^28.  Engine memory it keeps: with
+ * tokens_dev, 256 bytes a row and 8 for each 2048 logits or more of it, grown (after a
+ * stream synchronize) when a call needs more. */
 int tla_logits_process(tla_engine* e, int n_seq, int n_vocab, const tla_logit_rules* rules, float* out_dev,
                        const float* logits_dev, int* tokens_dev);
 
@@ -483,9 +489,11 @@ int tla_logits_process(tla_engine* e, int n_seq, int n_vocab, const tla_logit_ru
 enum tla_kernel_id {
     TLA_KERNEL_DECODE = 0,  /* split-KV decode attention (and forward()'s
                                short-context attention + W_o): RoPE + append +
-                               attention + split merge, one launch           */
+                               attention + split merge, one launch;
+                               tla_paged_attention's streamed rows           */
     TLA_KERNEL_PREFILL = 1, /* causal MFMA prefill attention (short prompts: with
-                               their RoPE + append, one launch); tla_paged_attention */
+                               their RoPE + append, one launch);
+                               tla_paged_attention's launches with chunks       */
     TLA_KERNEL_APPEND = 2,  /* prefill RoPE + cache append, as its own launch;
                                tla_paged_append                               */
     TLA_KERNEL_GEMV = 3,    /* projections: matmul / attn_qkv / attn_out /

@@ -66,10 +66,10 @@ __device__ __forceinline__ float ruled(float x, int count, float rep, float pres
 // (integer atomics, whose order does not show).  The logits and the first part
 // of the lists are requested before anything is waited for.
 //
-// Bound by memory: 8 bytes per logit.  200 x 100003 logits with all rules 45.6 us
-// and without any 31.2, a copy of them 31.4; the rest are the lists (5.1 us the
+// Bound by memory: 8 bytes per logit.  200 x 100003 logits with all rules 43.7 us
+// and without any 31.2, a copy of them 31.4; the rest are the lists (about 5 us the
 // history, 3.5 the biases, 2 the mask: each its loads, LDS atomics, a barrier) and
-// the rows' hand-over.  The hand-over passes no release or acquire: at device
+// the rows' hand-over.  64 x 32000 8.7 us, a copy 3.9: the same chain, once.  The hand-over passes no release or acquire: at device
 // scope those write back and drop the XCD's L2, in every workgroup (61 us became
 // 247).
 template <int kThreads, int kPer>

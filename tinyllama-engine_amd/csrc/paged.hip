@@ -1,5 +1,16 @@
 // Paged KV cache for gfx950: append of new keys (rotated) and values, and
 // attention of new tokens over their sequences' pages.
+//
+// Row r, a (token, head) pair with query q (rotated at its position p_r), over the
+// seen keys j <= p_r of its kv head (those in pages that are there):
+//     s_j = q . K_j / 8,  out = sum_j 2^(s_j log2 e - m) V_j / sum_j 2^(s_j log2 e - m).
+// One pass: m is a running maximum, and a part of the keys is the state (m, l, O);
+// two parts make one, O = O_a 2^(m_a - m) + O_b 2^(m_b - m) and l likewise.  All states
+// and sums are fp32.  A row that sees nothing has l = 0 and is 0.
+//
+// Single tokens are bound by memory (each key and value read once), chunks by the
+// matrix cores and the vector operations between their products: two kernels, and a
+// third that runs items of both.
 #include "bf16_split.h"
 #include "lane_math.h"
 #include "paged.h"
@@ -70,7 +81,12 @@ __device__ __forceinline__ long long row_of(const PagedPool& c, const int* table
     return row_in(c, table[pos >> c.page_shift], pos, kv_dim);
 }
 
-// One wave per token: its k and v rows in pieces of 4 floats, lanes over both.
+// One wave per token: its k and v rows in pieces of 4 floats, lanes over both.  k is
+// rotated with the operations of tla_rope, each rounded on its own: F32 pages hold its
+// bits, F16 and BF16 ones those rounded once, to nearest.  Bound by memory where
+// there are many tokens (BF16, 16 x 2048 tokens of 4 kv heads 21.3 us, 4.7 TB/s of the
+// 100.7 MB read and written; a copy reaches 5.05), by the launch where there are few (64
+// tokens 4.4 us a call, 3.8 in the kernel).
 template <int kType, int kMaxSeq>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendParams p, const PagedSeqs<kMaxSeq> b)
 {
@@ -463,6 +479,15 @@ struct StreamTile<kKvF32> {
 // them in order.  A wave holds one tile: its keys' registers take the next
 // tile's as soon as the scores are formed, its values' after P.V.  The other
 // waves of the SIMD cover the wait.
+//
+// Bound by memory: 64 sequences of 256 to 2047 F16 positions 19.0 us, 4.0 TB/s of
+// their 76.6 MB, of which about 4 us are the launch, the table and the query on their
+// way first and the parts' meeting last; 8 x 16384 F32 52.7 us, 5.1 TB/s, the rate of a
+// copy.  Four waves to a workgroup and one kv head: eight and sixteen waves, two and
+// four heads were slower or the same.  Parts are added by the last to arrive (a
+// second launch for it costs 3 us and more); their states go past the L2 to device
+// scope word by word, as a release and an acquire would write back and drop it (the
+// merge by plain loads after an acquire: 28 us for 20.7).
 // kSmall: pages of fewer than 16 positions: each lane looks up one row of the
 // next tile, and the lanes that load it ask that lane (BF16, pages of 8, 2
 // sequences of 15318: 17.0 us; 29 with ten look-ups by each lane as a tile's
@@ -892,6 +917,14 @@ struct ChunkTile<kKvF32> {
 // its waves share the tiles in LDS, double-buffered: the next one's rows are on
 // their way while the waves compute, directly into LDS (16-bit elements of large
 // pages) or in registers.
+//
+// Bound by issue: per 32 x 32 tile of F16 scores 16 matrix instructions of 32 cycles
+// stand beside about 130 vector ones of 4 (the exponentials 16), which overlap in
+// part only: in a chunk of 512 tokens after 8000 (82.7 us, 838 TFLOP/s of F16 pieces; a
+// large F16 matrix product reaches 1270) the matrix cores are busy 35 % of the
+// cycles and the vector units 40 %.  F32, a prompt of 2048: 111 us, 926 TFLOP/s of
+// BF16 pieces, 40 % and 40 %.  128 rows to a workgroup: 3 of them fit a CU, and their
+// 12 waves share 64 keys' reads.  The maximum is formed in few tiles only (below).
 // kSmall: pages of fewer than 8 positions, whose rows are looked up by each
 // lane; else the eight rows that a wave loads lie in one page.
 template <int kType>
@@ -1081,7 +1114,9 @@ __device__ __forceinline__ void chunk_item(const PagedAttentionParams& p, const 
     // the sum of a lane's 16 probabilities passes kLimit: most tiles form no
     // maximum and do not rescale O.  The scores are then formed once more (kAgain):
     // 16 registers fewer are live.  Not for F32, whose products are 3 to 6 times as
-    // many.
+    // many.  F16: a sum of 2^14 keeps every probability below F16's largest, and one
+    // at the maximum found last is 2^6; BF16 pieces need no such care, and 2^8 keeps
+    // the sums of many tiles far from fp32's end.
     float m_run = -INFINITY, l_run = 0.f, off = 0.f;
     constexpr float kShift = P::kShift;
     constexpr bool kAgain = kType != kKvF32;
@@ -1237,7 +1272,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
 }
 
 // Chunks and single tokens in one launch, the chunks' items first: either kind
-// alone seldom fills the GPU to its end.
+// alone seldom fills the GPU to its end (BF16, 32 sequences of up to 2047 positions, one
+// with 333 new tokens: 33.0 us in two launches, 26.3 in one).
 template <int kType, int kMaxSeq>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void paged_mixed_kernel(
     const PagedAttentionParams p, const PagedSeqs<kMaxSeq> chunks, const PagedSeqs<kMaxSeq> streams)
