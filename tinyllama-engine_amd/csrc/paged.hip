@@ -919,12 +919,13 @@ struct ChunkTile<kKvF32> {
 // pages) or in registers.
 //
 // Bound by issue: per 32 x 32 tile of F16 scores 16 matrix instructions of 32 cycles
-// stand beside about 130 vector ones of 4 (the exponentials 16), which overlap in
-// part only: in a chunk of 512 tokens after 8000 (82.7 us, 838 TFLOP/s of F16 pieces; a
-// large F16 matrix product reaches 1270) the matrix cores are busy 35 % of the
-// cycles and the vector units 40 %.  F32, a prompt of 2048: 111 us, 926 TFLOP/s of
-// BF16 pieces, 40 % and 40 %.  128 rows to a workgroup: 3 of them fit a CU, and their
-// 12 waves share 64 keys' reads.  The maximum is formed in few tiles only (below).
+// stand beside about 90 vector ones of 4 (the 16 exponentials of 16), and a SIMD runs
+// the two hardly at once: in a chunk of 512 tokens after 8000 (82.7 us, 838 TFLOP/s of
+// F16 pieces; a large F16 matrix product reaches 1270) the matrix cores are busy 41 %
+// of the cycles and the vector units 46 %.  F32, a prompt of 2048: 111 us, 926 TFLOP/s
+// of BF16 pieces, 44 % and 44 %.  128 rows to a workgroup: 3 of them fit
+// a CU, and their 12 waves share 64 keys' reads.  The maximum is formed in few tiles
+// only (below).
 // kSmall: pages of fewer than 8 positions, whose rows are looked up by each
 // lane; else the eight rows that a wave loads lie in one page.
 template <int kType>
@@ -1175,7 +1176,12 @@ __device__ __forceinline__ void chunk_item(const PagedAttentionParams& p, const 
                 e = weights(s);
             }
             l_run += sum;
+            // P.V before the SIMD's other waves' vector operations (F16, 4 x 1500 tokens
+            // 103.9 -> 99.8 us, F32 512 after 8000 192 -> 185; raised for the scores too,
+            // or for the vector operations instead, neither gained).
+            __builtin_amdgcn_s_setprio(1);
             Tile::accumulate(e, s_kv[buf][u], v_at, o);
+            __builtin_amdgcn_s_setprio(0);
         }
         if (tile + 1 < tile_end) store(buf ^ 1);
         __syncthreads();
