@@ -60,25 +60,27 @@ __device__ __forceinline__ float ruled(float x, int count, float rep, float pres
     return x;
 }
 
-// One workgroup per slice of 4 kPer x kThreads logits of a row.  The slice's counts
-// of the history's tokens, then the places of its last biases are gathered in
-// LDS, one word per logit: every workgroup of a row reads the row's lists
-// (integer atomics, whose order does not show).  The logits and the first part
-// of the lists are requested before anything is waited for.
+// One workgroup per slice of 4 kPer x kThreads logits of a row.  The counts of the
+// history's tokens in the slice and the places of its last biases are gathered in
+// LDS, a word of each per logit: every workgroup of a row reads the row's lists
+// (integer atomics, whose order does not show).  The logits and the first parts of
+// the lists, the biases' values too, are requested before anything is waited for.
 //
-// Bound by memory: 8 bytes per logit.  200 x 100003 logits with all rules 43.7 us
-// and without any 31.2, a copy of them 31.4; the rest are the lists (about 5 us the
-// history, 3.5 the biases, 2 the mask: each its loads, LDS atomics, a barrier) and
-// the rows' hand-over.  64 x 32000 8.7 us, a copy 3.9: the same chain, once.  The hand-over passes no release or acquire: at device
-// scope those write back and drop the XCD's L2, in every workgroup (61 us became
-// 247).
+// Bound by memory: 8 bytes per logit.  200 x 100003 logits with all rules 42.3 us
+// and without any 31.2, a copy of them 31.4; the rest are the lists (about 4 us the
+// history, 3 the biases, 2 the mask: loads, LDS atomics, a barrier) and the rows'
+// hand-over.  64 x 32000 8.4 us, a copy 3.9: the same chain, once.  (One array for
+// both lists, one after the other, and the values loaded when their places are known:
+// 43.9 and 8.8 us.)  The hand-over passes no release or acquire: at device scope
+// those write back and drop the XCD's L2, in every workgroup (61 us became 247).
 template <int kThreads, int kPer>
 __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsParams p)
 {
     constexpr int kSlice = 4 * kPer * kThreads;
-    __shared__ int4 s_word4[kPer * kThreads];
+    __shared__ int4 s_count4[kPer * kThreads];  // how often the history holds each logit's token
+    __shared__ int4 s_place4[kPer * kThreads];  // 1 + the place of its last bias, 0: none
     __shared__ unsigned long long s_best[kThreads / 64];
-    int* const s_word = reinterpret_cast<int*>(s_word4);
+    __shared__ float s_value[kThreads];  // the first biases
     const int tid = threadIdx.x;
     const int row = blockIdx.x / p.n_slices, slice = blockIdx.x % p.n_slices;
     const int j0 = slice * kSlice, n = min(kSlice, p.n_vocab - j0);
@@ -101,66 +103,69 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsParams p)
     }
     const int* const h = r.history_dev + (long long)row * r.history_stride;
     const int* const t = r.bias_token_dev + (long long)row * r.bias_stride;
-    int h_len = 0, b_len = 0, h0 = -1, t0 = -1;
-    float rep = 1.f, pres = 0.f, freq = 0.f;
+    int h_len = 0, b_len = 0, h0 = -1, h1 = -1, t0 = -1;
+    float rep = 1.f, pres = 0.f, freq = 0.f, b0 = 0.f;
     if (r.history_dev) {
         if (tid < r.history_stride) h0 = h[tid];
+        if (tid + kThreads < r.history_stride) h1 = h[tid + kThreads];
         h_len = min(max(r.history_len_dev[row], 0), r.history_stride);
         rep = r.penalties_dev[3 * (long long)row];
         pres = r.penalties_dev[3 * (long long)row + 1];
         freq = r.penalties_dev[3 * (long long)row + 2];
     }
     if (r.bias_token_dev) {
-        if (tid < r.bias_stride) t0 = t[tid];
+        if (tid < r.bias_stride) {
+            t0 = t[tid];
+            b0 = r.bias_value_dev[(long long)row * r.bias_stride + tid];
+        }
         b_len = min(max(r.bias_len_dev[row], 0), r.bias_stride);
     }
     if (r.history_dev || r.bias_token_dev) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) s_word4[tid + kThreads * i] = make_int4(0, 0, 0, 0);
-        __syncthreads();
-    }
-    if (r.history_dev) {  // the words count
-        const auto add = [&](int token) {
-            const unsigned j = (unsigned)token - (unsigned)j0;
-            if (j < (unsigned)n) atomicAdd(&s_word[j], 1);
-        };
-        if (tid < h_len) add(h0);
-        for (int i = tid + kThreads; i < h_len; i += 4 * kThreads) {  // four loads in flight
-            int k[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) k[u] = i + u * kThreads < h_len ? h[i + u * kThreads] : -1;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) add(k[u]);
+        for (int i = 0; i < kPer; ++i) {
+            s_count4[tid + kThreads * i] = make_int4(0, 0, 0, 0);
+            s_place4[tid + kThreads * i] = make_int4(0, 0, 0, 0);
         }
+        s_value[tid] = b0;
         __syncthreads();
+        if (r.history_dev) {
+            const auto add = [&](int token) {
+                const unsigned j = (unsigned)token - (unsigned)j0;
+                if (j < (unsigned)n) atomicAdd(&reinterpret_cast<int*>(s_count4)[j], 1);
+            };
+            if (tid < h_len) add(h0);
+            if (tid + kThreads < h_len) add(h1);
+            for (int i = tid + 2 * kThreads; i < h_len; i += 4 * kThreads) {  // four loads in flight
+                int k[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) k[u] = i + u * kThreads < h_len ? h[i + u * kThreads] : -1;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) add(k[u]);
+            }
+        }
+        if (r.bias_token_dev)
+            for (int i = tid; i < b_len; i += kThreads) {
+                const unsigned j = (unsigned)(i == tid ? t0 : t[i]) - (unsigned)j0;
+                if (j < (unsigned)n) atomicMax(&reinterpret_cast<int*>(s_place4)[j], i + 1);
+            }
+        __syncthreads();
+        const float* const value = r.bias_value_dev + (long long)row * r.bias_stride - 1;
+        const auto bias = [&](int place) { return place <= kThreads ? s_value[place - 1] : value[place]; };
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int4 c = s_word4[tid + kThreads * i];
+            const int4 c = s_count4[tid + kThreads * i];
             if (c.x | c.y | c.z | c.w) {
                 v[i][0] = ruled(v[i][0], c.x, rep, pres, freq);
                 v[i][1] = ruled(v[i][1], c.y, rep, pres, freq);
                 v[i][2] = ruled(v[i][2], c.z, rep, pres, freq);
                 v[i][3] = ruled(v[i][3], c.w, rep, pres, freq);
-                s_word4[tid + kThreads * i] = make_int4(0, 0, 0, 0);
             }
-        }
-        __syncthreads();
-    }
-    if (r.bias_token_dev) {  // 1 + the place of the last bias of the token
-        for (int i = tid; i < b_len; i += kThreads) {
-            const unsigned j = (unsigned)(i == tid ? t0 : t[i]) - (unsigned)j0;
-            if (j < (unsigned)n) atomicMax(&s_word[j], i + 1);
-        }
-        __syncthreads();
-        const float* const value = r.bias_value_dev + (long long)row * r.bias_stride - 1;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int4 c = s_word4[tid + kThreads * i];
-            if (c.x | c.y | c.z | c.w) {
-                if (c.x) v[i][0] += value[c.x];
-                if (c.y) v[i][1] += value[c.y];
-                if (c.z) v[i][2] += value[c.z];
-                if (c.w) v[i][3] += value[c.w];
+            const int4 b = s_place4[tid + kThreads * i];
+            if (b.x | b.y | b.z | b.w) {
+                if (b.x) v[i][0] += bias(b.x);
+                if (b.y) v[i][1] += bias(b.y);
+                if (b.z) v[i][2] += bias(b.z);
+                if (b.w) v[i][3] += bias(b.w);
             }
         }
     }
