@@ -919,13 +919,13 @@ struct ChunkTile<kKvF32> {
 // pages) or in registers.
 //
 // Bound by issue: per 32 x 32 tile of F16 scores 16 matrix instructions of 32 cycles
-// stand beside about 90 vector ones of 4 (the 16 exponentials of 16), and a SIMD runs
-// the two hardly at once: in a chunk of 512 tokens after 8000 (82.7 us, 838 TFLOP/s of
-// F16 pieces; a large F16 matrix product reaches 1270) the matrix cores are busy 41 %
-// of the cycles and the vector units 46 %.  F32, a prompt of 2048: 111 us, 926 TFLOP/s
-// of BF16 pieces, 44 % and 44 %.  128 rows to a workgroup: 3 of them fit
-// a CU, and their 12 waves share 64 keys' reads.  The maximum is formed in few tiles
-// only (below).
+// stand beside about 90 vector ones of 4 (the 16 exponentials of 16), and a SIMD
+// overlaps the two in part only: in a chunk of 512 tokens after 8000 (82.7 us, 838
+// TFLOP/s of F16 pieces; a large F16 matrix product reaches 1270) the matrix cores are
+// busy 41 % of the cycles and the vector units 46 %.  F32, a prompt of 2048: 111 us, 926
+// TFLOP/s of BF16 pieces, 44 % and 44 %.  128 rows to a workgroup: 3 of them fit a CU,
+// and their 12 waves share 64 keys' reads.  The maximum is formed in few tiles only
+// (below).
 // kSmall: pages of fewer than 8 positions, whose rows are looked up by each
 // lane; else the eight rows that a wave loads lie in one page.
 template <int kType>
